@@ -5,6 +5,7 @@ Layout:
                       built into libparoquant_hip.so by build.py
   _lib.py             ctypes binding of the C ABI
   ops.py              torch custom ops (rotation::rotate, paroquant::*)
+  attention.py        attention and the paged int8 cache (paroquant_attn::*)
   paroquant_kernels/  drop-in for the reference's kernels/paroquant_kernels
   quantization/       drop-in for src/alpamayo_r1/utils/quantization
   workloads.py        seeded synthetic inputs of the benchmark configurations
@@ -25,6 +26,6 @@ if _os.path.exists(_lib.LIB_PATH):
 elif _torch.cuda.is_available():
     raise ImportError(f"{_lib.LIB_PATH} is missing: build it with `python alpamayo_amd/build.py`")
 
-from . import ops  # noqa: E402,F401
+from . import attention, ops  # noqa: E402,F401
 
-__all__ = ["ops"]
+__all__ = ["attention", "ops"]

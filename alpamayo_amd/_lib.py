@@ -32,6 +32,7 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _UINT = ctypes.c_uint
 _SZ = ctypes.c_size_t
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/paroquant_hip.h
 class LinearMember(ctypes.Structure):
@@ -87,6 +88,12 @@ SIGNATURES = {
     "pq_w4a16_linear_workspace_size": (_SZ, [_I64, _I64]),
     "pq_w4a16_linear": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _P, _INT, _P, _INT, _I64, _I64, _I64, _INT, _UINT, _P,
                                _SZ, _P]),
+    "pq_attn_prompt": (_INT, [_P, _P, _P, _INT, *[_I64] * 6, _P, _P, _P, _P, *[_I64] * 6, _F, _INT, _P]),
+    "pq_kv_append_i8": (_INT, [_P, _P, _INT, *[_I64] * 4, *[_P] * 7, *[_I64] * 6, _P]),
+    "pq_attn_cache_i8_workspace_size": (_SZ, [_I64] * 4),
+    "pq_attn_cache_i8": (_INT, [_P, _INT, _I64, _I64, *[_P] * 9, *[_I64] * 7, _F, _P, _SZ, _P]),
+    "pq_attn_cache_weights_i8": (_INT, [_P, _INT, _I64, _I64, *[_P] * 7, *[_I64] * 8, _F, _P]),
+    "pq_kv_evict_i8": (_INT, [*[_P] * 11, *[_I64] * 9, _P]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,123 @@
+// Device helpers shared by the attention and cache kernels: packed sequences,
+// pages of the int8 cache, 16-bit floats and reductions over lanes.
+#pragma once
+
+#include "pq_common.h"
+
+namespace pqa {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+constexpr int kPage = 64;             // tokens of a cache page
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// A page whose largest value is below this holds zeros: 1 / (its scale) stays finite.
+constexpr float kTiny = 0x1p-100f;
+
+__device__ __forceinline__ int lane_id() { return static_cast<int>(threadIdx.x & 63); }
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
+
+// The other half of the wave's value combined with the own: every lane ends with both.
+__device__ __forceinline__ float max_xor32(float x) {
+  const u2 r = __builtin_bit_cast(
+      u2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_xor32(float x) {
+  const u2 r = __builtin_bit_cast(
+      u2, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The same over neighbouring groups of 16 lanes.
+__device__ __forceinline__ float max_xor16(float x) {
+  const u2 r = __builtin_bit_cast(
+      u2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_xor16(float x) {
+  const u2 r = __builtin_bit_cast(
+      u2, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---------------------------------------------------------------------------
+// Packed sequences.  Lengths live on the device only, so that no call waits
+// for them and a captured graph serves other lengths; every index read from
+// the device is brought into its tensor's range before it is used.
+// ---------------------------------------------------------------------------
+
+struct Span { int first, count; };
+
+// Rows [first, first + count) of sequence b of a packed tensor of `total` rows.
+__device__ __forceinline__ Span span_of(const int* cu, int b, int total) {
+  const int lo = min(max(cu[b], 0), total), hi = min(max(cu[b + 1], lo), total);
+  return {lo, hi - lo};
+}
+
+struct Found { int b; int64_t local; };   // b < 0: past the last one
+
+// The sequence in which number idx of the numbers cost(0) + cost(1) + ... lies, by all lanes of a wave: each takes one
+// sequence of 64 at a time.
+template <class F>
+__device__ __forceinline__ Found find_seq(int batch, int64_t idx, F cost) {
+  const int lane = lane_id();
+  int64_t before = 0;
+  for (int base = 0; base < batch; base += 64) {
+    const int b = base + lane;
+    const int64_t own = b < batch ? cost(b) : 0;
+    int64_t incl = own;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int64_t up = __shfl_up(incl, s);
+      if (lane >= s) incl += up;
+    }
+    const uint64_t past = __ballot(idx < before + incl);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      return {base + at, idx - before - __shfl(incl - own, at)};
+    }
+    before += __shfl(incl, 63);
+  }
+  return {-1, idx - before};
+}
+
+template <class F>
+__device__ __forceinline__ int64_t sum_seqs(int batch, F cost) {
+  int64_t sum = 0;
+  for (int b = lane_id(); b < batch; b += 64) sum += cost(b);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+  return sum;
+}
+
+// ---------------------------------------------------------------------------
+// int8 codes as fp16, eight at a time: c + 128 in the low byte of 0x64xx is
+// the fp16 1024 + 128 + c, and the difference to 1152 is c without rounding.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ h8 codes_f16(uint32_t lo, uint32_t hi) {
+  const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
+  const h2 off = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+  union { h2 p[4]; h8 v; } r;
+  r.p[0] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) - off;
+  r.p[1] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) - off;
+  r.p[2] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - off;
+  r.p[3] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - off;
+  return r.v;
+}
+
+__device__ __forceinline__ int code_of(float x, float inv) {
+  // NaN holds the place of a zero; infinities saturate
+  const float r = __builtin_rintf(x * inv);
+  return x != x ? 0 : static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
+}
+
+}  // namespace pqa

@@ -1,0 +1,301 @@
+// prompt_attention: causal attention over packed prompts with grouped heads.
+//
+//   s_ij = scale * q_i . k_j,  o_i = sum_j p_ij v_j / sum_j p_ij,  p = exp(s - max)
+//
+// One pass over the keys with the running maximum and sum of each row.  A
+// workgroup carries 128 rows, 32 a wave; a key/value head's rows are its
+// (token, query head) pairs, so the query heads of a group share the keys and
+// values that the workgroup stages in LDS, 64 at a time.
+//
+// Both products are taken transposed: S^T = K Q^T, O^T = V^T P^T.  A lane then
+// holds scores of one row (column lane & 31), its maximum needs one exchange
+// with the other half of the wave and rescaling none.  The keys are dealt to
+// the rows of S^T such that the scores a lane holds, rounded to 16 bits, are
+// the second product's operand as they stand.  V^T comes from LDS through the
+// transposing reads.
+//
+// p is rounded to the inputs' type (half a step 2^-9 of the value in bf16,
+// 2^-12 in fp16, as the outputs are); scores, sums and statistics are float32.
+#include <algorithm>
+
+#include "pq_attn.h"
+#include "pq_device.h"
+
+namespace {
+
+using namespace pqa;
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kRows = 32 * kWaves;
+constexpr int kKeys = 64;
+
+struct PromptArgs {
+  const uint16_t* q;         // [tokens_q, heads * group, d]
+  const uint16_t* k;         // [tokens_k, heads, d]
+  const uint16_t* v;
+  uint16_t* out;             // [tokens_q, heads * group, d]
+  float* lse;                // [heads * group, tokens_q]
+  const int* cu_q;           // [batch + 1]
+  const int* cu_k;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+  int batch, tokens_q, tokens_k, heads, group, tiles, causal;
+  float scale_log2;
+};
+
+// 16-byte chunk c of row r lies at place c ^ swz(r) of the row: rows that are read together, 4 in a transposing read
+// and 16 in a plain one, start in different banks.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (D == 128) return (r & 3) << 2 | (r >> 2 & 3);
+  else return (r >> 1 & 1) << 2 | (r >> 2 & 3);
+}
+
+template <bool BF16>
+__device__ __forceinline__ f16v mfma32(s8 a, s8 b, f16v c) {
+  if constexpr (BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF16) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
+  } else {
+    return pqd::pk_f16(a, b);
+  }
+}
+
+// Copies kKeys rows from row k0 on (past the last: the last again) to LDS, swizzled.
+template <int D>
+__device__ __forceinline__ void stage(const uint16_t* base, int64_t stride, int k0, int last, uint16_t* lds) {
+  constexpr int kChunks = D / 8, kEach = kKeys * kChunks / kThreads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int at = (wave * kEach + i) * 64, c = (at + lane) % kChunks, r = (at + lane) / kChunks;
+    const uint16_t* src = base + static_cast<int64_t>(min(k0 + r, last)) * stride + (c ^ swz<D>(r)) * 8;
+    pqd::lds_copy16(src, pqd::lds_addr(lds) + at * 16);
+  }
+}
+
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) {
+  constexpr int kDt = D / 32, kSteps = D / 16;
+  __shared__ __align__(16) uint16_t ks[kKeys * D], vs[kKeys * D];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, col = lane & 31;
+  const int head = blockIdx.x % a.heads;
+  const int idx = a.tiles - 1 - blockIdx.x / a.heads;   // late rows of a prompt see most keys: they start first
+
+  const Found f = find_seq(a.batch, idx, [&](int b) -> int64_t {
+    return (static_cast<int64_t>(span_of(a.cu_q, b, a.tokens_q).count) * a.group + kRows - 1) / kRows;
+  });
+  if (f.b < 0) {
+    // the workgroups left over clear the rows outside of the sequences
+    const int lo = a.batch > 0 ? min(max(a.cu_q[0], 0), a.tokens_q) : 0;
+    const int hi = a.batch > 0 ? max(lo, min(max(a.cu_q[a.batch], 0), a.tokens_q)) : 0;
+    const int rest = a.tokens_q - (hi - lo), left = a.tiles - (idx - static_cast<int>(f.local));
+    for (int i = static_cast<int>(f.local); i < rest; i += left) {
+      const int token = i < lo ? i : hi + i - lo;
+      uint16_t* op = a.out + (static_cast<int64_t>(token) * a.heads + head) * a.group * D;
+      for (int c = t; c < a.group * D; c += kThreads) op[c] = 0;
+      for (int g = t; g < a.group; g += kThreads)
+        a.lse[(static_cast<int64_t>(head) * a.group + g) * a.tokens_q + token] = -INFINITY;
+    }
+    return;
+  }
+  const Span sq = span_of(a.cu_q, f.b, a.tokens_q), sk = span_of(a.cu_k, f.b, a.tokens_k);
+  const int rows = sq.count * a.group, row0 = static_cast<int>(f.local) * kRows, shift = sk.count - sq.count;
+  // keys that a row of token i sees
+  const auto sees = [&](int i) { return a.causal ? max(0, min(i + shift + 1, sk.count)) : sk.count; };
+
+  const int row = row0 + wave * 32 + col;
+  const bool valid = row < rows;
+  const int token = valid ? row / a.group : 0, h = valid ? row - token * a.group : 0;
+  const int limit = valid ? sees(token) : 0;
+  const int end = sees((min(row0 + kRows, rows) - 1) / a.group);
+  const int wrow = row0 + wave * 32;
+  const int wend = wrow < rows ? sees((min(wrow + 32, rows) - 1) / a.group) : 0;   // keys that the wave's rows see
+  const int sure = wrow < rows ? sees(wrow / a.group) : 0;                         // that all of them see
+
+  s8 qf[kSteps];
+  {
+    const uint16_t* p = a.q + (sq.first + token) * a.q_st + (static_cast<int64_t>(head) * a.group + h) * a.q_sh + 8 * half;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      qf[i] = s8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (valid) qf[i] = *reinterpret_cast<const s8*>(p + 16 * i);
+    }
+  }
+  const uint16_t* kb = a.k + sk.first * a.k_st + head * a.k_sh;
+  const uint16_t* vb = a.v + sk.first * a.v_st + head * a.v_sh;
+
+  f16v o[kDt];
+#pragma unroll
+  for (int i = 0; i < kDt; ++i) o[i] = f16v{};
+  float m = -INFINITY, l = 0.0f;
+  const float c = a.scale_log2;
+
+  // K: the lane's row of S^T is key kr (bits 2 and 3 of the row swapped), chunk 2 s + half in step s
+  const int kr = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;
+  // V: the lane's address in a transposing read of 4 keys by 16 channels
+  const int l16 = lane & 15, vsub = lane >> 4 & 1;
+
+  for (int k0 = 0; k0 < end; k0 += kKeys) {
+    stage<D>(kb, a.k_st, k0, sk.count - 1, ks);
+    stage<D>(vb, a.v_st, k0, sk.count - 1, vs);
+    pqd::wait_vmcnt<0>();
+    __syncthreads();
+    if (k0 < wend) {
+      f16v s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = f16v{};
+        const int r = 32 * u + kr;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+          s[u] = mfma32<BF16>(*reinterpret_cast<const s8*>(ks + r * D + ((2 * i + half) ^ swz<D>(r)) * 8), qf[i], s[u]);
+      }
+      const bool masked = k0 + kKeys > sure;
+      float big = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (masked && k0 + 32 * u + 16 * (i >> 3) + 8 * half + (i & 7) >= limit) s[u][i] = -INFINITY;
+          big = fmaxf(big, s[u][i]);
+        }
+      big = fmaxf(m, max_xor32(big) * c);
+      const float base = big == -INFINITY ? 0.0f : big;
+      const float alpha = exp2_fast(m - base);
+      m = big;
+      float sum = 0.0f;
+      s8 pf[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float x = exp2_fast(__builtin_fmaf(s[u][i], c, -base)), y = exp2_fast(__builtin_fmaf(s[u][i + 1], c, -base));
+          sum += x + y;
+          const uint32_t w = pack2<BF16>(x, y);
+          pf[2 * u + (i >> 3)][i & 7] = static_cast<short>(w & 0xffffu);
+          pf[2 * u + (i >> 3)][(i & 7) + 1] = static_cast<short>(w >> 16);
+        }
+      l = l * alpha + sum;
+#pragma unroll
+      for (int i = 0; i < kDt; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+
+      // In a masked tile a value that is not finite must not meet the weight 0 of a row that does not see its key:
+      // there it takes no part in the product and is added to the rows that do see it.
+      bool odd = false;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < kDt; ++i) {
+          s8 vf;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int r = 16 * u + 8 * half + 4 * x + (l16 >> 2);
+            const int ch = (4 * i + 2 * vsub + (l16 >> 1 & 1)) ^ swz<D>(r);
+            const s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s4*)(vs + r * D + ch * 8 + (l16 & 1) * 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vf[4 * x + e] = w[e];
+          }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              constexpr int kInf = BF16 ? 0x7f80 : 0x7c00;
+              const bool bad = (vf[e] & kInf) == kInf;
+              odd |= bad;
+              vf[e] = bad ? static_cast<short>(0) : vf[e];
+            }
+          }
+          o[i] = mfma32<BF16>(vf, pf[u], o[i]);
+        }
+      if (masked && __ballot(odd)) {
+        for (int key = 0; key < kKeys && k0 + key < sk.count; ++key) {
+          if (k0 + key >= limit) continue;
+#pragma unroll
+          for (int i = 0; i < kDt; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int d = 32 * i + (e & 3) + 8 * (e >> 2) + 4 * half;
+              const float x = pq_raw_to_f32<BF16 ? PQ_BF16 : PQ_F16>(vs[key * D + (((d >> 3) ^ swz<D>(key)) << 3) + (d & 7)]);
+              if (!(fabsf(x) < INFINITY)) o[i][e] += x;
+            }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  l = sum_xor32(l);
+  if (!valid) return;
+  const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+  uint16_t* op = a.out + ((static_cast<int64_t>(sq.first) + token) * a.heads * a.group + head * a.group + h) * D;
+#pragma unroll
+  for (int i = 0; i < kDt; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<uint2*>(op + 32 * i + 2 * e + 4 * half) =
+          make_uint2(pack2<BF16>(o[i][e] * inv, o[i][e + 1] * inv), pack2<BF16>(o[i][e + 2] * inv, o[i][e + 3] * inv));
+  if (half == 0)
+    a.lse[(static_cast<int64_t>(head) * a.group + h) * a.tokens_q + sq.first + token] = (m + log2_fast(l)) * kLn2;
+}
+
+}  // namespace
+
+extern "C" int pq_attn_prompt(const void* q, const void* k, const void* v, int dtype, int64_t q_stride_token,
+                              int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head,
+                              int64_t v_stride_token, int64_t v_stride_head, const int32_t* cu_seqlens_q,
+                              const int32_t* cu_seqlens_k, void* out, float* lse, int64_t batch, int64_t tokens_q,
+                              int64_t tokens_k, int64_t kv_heads, int64_t group, int64_t head_dim, float scale,
+                              int causal, void* stream) {
+  const char* who = "pq_attn_prompt";
+  PQ_REQUIRE(dtype == PQ_F16 || dtype == PQ_BF16, PQ_ERR_UNSUPPORTED, "%s: dtype code %d (Half or BFloat16)", who, dtype);
+  PQ_REQUIRE(head_dim == 64 || head_dim == 128, PQ_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 64, 128)", who,
+             (long long)head_dim);
+  PQ_REQUIRE(kv_heads >= 1 && group >= 1 && kv_heads * group <= 65535, PQ_ERR_ARG, "%s: kv_heads=%lld group=%lld", who,
+             (long long)kv_heads, (long long)group);
+  PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffLL && tokens_q >= 0 && tokens_k >= 0 && tokens_k <= 0x7fffffffLL - 64 &&
+                 tokens_q * group <= 0x7fffffffLL - kRows, PQ_ERR_ARG,
+             "%s: batch=%lld tokens_q=%lld tokens_k=%lld", who, (long long)batch, (long long)tokens_q, (long long)tokens_k);
+  PQ_REQUIRE(scale > 0.0f && scale < INFINITY, PQ_ERR_ARG, "%s: scale=%g must be positive and finite", who, scale);
+  if (tokens_q == 0) return PQ_OK;
+  PQ_REQUIRE(q && out && lse && (tokens_k == 0 || (k && v)) && (batch == 0 || (cu_seqlens_q && cu_seqlens_k)), PQ_ERR_ARG,
+             "%s: null pointer", who);
+  PQ_REQUIRE(pq::aligned_to(q, 16) && pq::aligned_to(k, 16) && pq::aligned_to(v, 16) && pq::aligned_to(out, 16), PQ_ERR_ARG,
+             "%s: q, k, v and out must be 16-byte aligned", who);
+  PQ_REQUIRE(q_stride_token % 8 == 0 && q_stride_head % 8 == 0 && k_stride_token % 8 == 0 && k_stride_head % 8 == 0 &&
+                 v_stride_token % 8 == 0 && v_stride_head % 8 == 0, PQ_ERR_ARG,
+             "%s: strides must be multiples of 8 values", who);
+  PromptArgs a;
+  a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<uint16_t*>(out); a.lse = lse; a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k;
+  a.q_st = q_stride_token; a.q_sh = q_stride_head; a.k_st = k_stride_token; a.k_sh = k_stride_head;
+  a.v_st = v_stride_token; a.v_sh = v_stride_head;
+  a.batch = static_cast<int>(batch); a.tokens_q = static_cast<int>(tokens_q); a.tokens_k = static_cast<int>(tokens_k);
+  a.heads = static_cast<int>(kv_heads); a.group = static_cast<int>(group); a.causal = causal != 0;
+  a.scale_log2 = scale * kLog2e;
+  // tiles of all sequences, each of which may end inside one, and one for the rows outside of them
+  const int64_t tiles = tokens_q * group / kRows + std::min<int64_t>(batch, tokens_q) + 1;
+  PQ_REQUIRE(tiles * kv_heads <= 0x7fffffffLL, PQ_ERR_ARG, "%s: too many rows", who);
+  a.tiles = static_cast<int>(tiles);
+  const unsigned grid = static_cast<unsigned>(tiles * kv_heads);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (head_dim == 64 && dtype == PQ_BF16) attn_prompt_kernel<64, true><<<grid, kThreads, 0, s>>>(a);
+  else if (head_dim == 64) attn_prompt_kernel<64, false><<<grid, kThreads, 0, s>>>(a);
+  else if (dtype == PQ_BF16) attn_prompt_kernel<128, true><<<grid, kThreads, 0, s>>>(a);
+  else attn_prompt_kernel<128, false><<<grid, kThreads, 0, s>>>(a);
+  return pq::launch_status("pq_attn_prompt launch");
+}

@@ -1,0 +1,225 @@
+// kv_append_i8: the keys and values of new tokens into the paged int8 cache.
+//
+// A page holds 64 tokens; it has one float32 scale for each key/value head
+// and side (keys, values), its absmax / 127, and code = round(x / scale).
+// K codes lie [64][d], V codes transposed [d][64]: the attention over the
+// cache takes both operands of its products as 16-byte runs of a row.
+//
+// Where new tokens of a page are larger than what it holds, its scale grows
+// and its codes are rounded to it: round(code * old / new), at most half a
+// step of the new scale each time.  A page whose first token is new holds
+// nothing: what its memory held before does not count.  The scale comes from
+// finite values only, so one bad value does not wipe out its page: infinities
+// saturate, NaN is held as 0.
+//
+// One workgroup per touched page, head and side; no two write the same page
+// side.  Every byte of a page outside of what is written stays as it was.
+#include "pq_attn.h"
+
+namespace {
+
+using namespace pqa;
+
+constexpr int kThreads = 256;
+
+struct AppendArgs {
+  const void* x[2];          // K, V rows [tokens, heads, d]
+  int8_t* cache[2];          // [pages, heads, 64, d], [pages, heads, d, 64]
+  float* scale[2];           // [pages, heads]
+  int64_t st[2], sh[2];      // strides of a token and of a head, in values
+  const int* table;          // [batch, width]
+  const int* cu;             // [batch + 1]
+  const int* cached;         // [batch]
+  int batch, width, tokens, heads, pages;
+};
+
+__device__ __forceinline__ int cached_len(const AppendArgs& a, int b) { return max(a.cached[b], 0); }
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
+  if constexpr (DT == PQ_F32) {
+    const f4* q = reinterpret_cast<const f4*>(static_cast<const float*>(p) + i);
+    const f4 a = q[0], b = q[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+  } else {
+    const u4 w = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = pq_raw_to_f32<DT>(w[j] & 0xffffu);
+      v[2 * j + 1] = pq_raw_to_f32<DT>(w[j] >> 16);
+    }
+  }
+}
+
+// The bytes of a dword scaled by `ratio` and rounded.
+__device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = static_cast<int8_t>(w >> (8 * j));
+    r |= (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(static_cast<float>(c) * ratio))) & 0xffu) << (8 * j);
+  }
+  return r;
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendArgs a) {
+  constexpr int kChunks = D / 8;                        // 8 values of a row for each thread
+  constexpr int kRows = kPage * kChunks / kThreads;     // neighbouring rows of a thread: 4 (d = 128) or 2
+  constexpr int kPitch = kPage + 4;
+  __shared__ uint32_t top[4];
+  __shared__ __align__(16) uint8_t tile[D * kPitch];
+
+  const int side = blockIdx.z, head = blockIdx.y, t = threadIdx.x;
+  const Found f = find_seq(a.batch, blockIdx.x, [&](int b) -> int64_t {
+    const int n = span_of(a.cu, b, a.tokens).count;
+    return n > 0 ? (static_cast<int64_t>(n) + cached_len(a, b) % kPage + kPage - 1) / kPage : 0;
+  });
+  if (f.b < 0) return;
+  const Span rows = span_of(a.cu, f.b, a.tokens);
+  const int64_t held = cached_len(a, f.b);
+  const int64_t j = held / kPage + f.local;
+  if (j >= a.width) return;
+  const int page = a.table[static_cast<int64_t>(f.b) * a.width + j];
+  if (page < 0 || page >= a.pages) return;
+  const int64_t first = j * kPage > held ? j * kPage : held;
+  const int64_t end = (j + 1) * kPage < held + rows.count ? (j + 1) * kPage : held + rows.count;
+  const int slot = static_cast<int>(first - j * kPage), count = static_cast<int>(end - first);
+  const int64_t row0 = rows.first + (first - held);
+
+  const int64_t ph = static_cast<int64_t>(page) * a.heads + head;
+  int8_t* cache = a.cache[side] + ph * (kPage * D);
+  float* scale = a.scale[side] + ph;
+
+  const int c = t % kChunks, r0 = t / kChunks * kRows;
+  float v[kRows][8];
+  uint32_t big = 0;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    // page slot r0 + r; outside of the new tokens it takes zeros
+    const int i = r0 + r - slot;
+    if (i >= 0 && i < count) {
+      load8<DT>(a.x[side], (row0 + i) * a.st[side] + head * a.sh[side] + c * 8, v[r]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[r][q] = 0.0f;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t m = __float_as_uint(v[r][q]) & 0x7fffffffu;
+      big = m < 0x7f800000u && m > big ? m : big;
+    }
+  }
+  big = pq_wave_umax(big);
+  if ((t & 63) == 0) top[t >> 6] = big;
+  const float old = slot > 0 ? *scale : 0.0f;
+  __syncthreads();
+  const float amax = __uint_as_float(max(max(top[0], top[1]), max(top[2], top[3])));
+  const float fresh = amax < kTiny ? 0.0f : amax / 127.0f;
+  const bool grown = fresh > old;
+  const float now = grown ? fresh : old;
+  const float inv = now > 0.0f ? 1.0f / now : 0.0f;
+  const bool redo = grown && slot > 0;
+  const float ratio = redo ? old / now : 1.0f;
+
+  if (side == 0) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int i = r0 + r - slot;
+      if (i < 0 || i >= count) continue;
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) w[q >> 2] |= (static_cast<uint32_t>(code_of(v[r][q], inv)) & 0xffu) << (8 * (q & 3));
+      *reinterpret_cast<uint2*>(cache + (r0 + r) * D + c * 8) = make_uint2(w[0], w[1]);
+    }
+    if (redo) {
+      for (int q = t; q < slot * D / 4; q += kThreads) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(cache) + q;
+        *p = requant4(*p, ratio);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) w |= (static_cast<uint32_t>(code_of(v[r][q], inv)) & 0xffu) << (8 * r);
+      uint8_t* p = tile + (c * 8 + q) * kPitch + r0;
+      if constexpr (kRows == 4) *reinterpret_cast<uint32_t*>(p) = w;
+      else *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w);
+    }
+    __syncthreads();
+    // 16 tokens of a channel at a time: new codes, held ones (rounded anew where the scale grew), and what lies behind
+    for (int q = t; q < D * 4; q += kThreads) {
+      const int d = q >> 2, t0 = (q & 3) * 16;
+      if (t0 >= slot + count || (t0 + 16 <= slot && !redo)) continue;
+      u4* p = reinterpret_cast<u4*>(cache + d * kPage + t0);
+      u4 w = {0, 0, 0, 0};
+      if (t0 < slot || t0 + 16 > slot + count) w = *p;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t nw = *reinterpret_cast<const uint32_t*>(tile + d * kPitch + t0 + 4 * k);
+        const uint32_t was = redo ? requant4(w[k], ratio) : w[k];
+        uint32_t r = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = t0 + 4 * k + e;
+          const uint32_t from = at < slot ? was : at < slot + count ? nw : w[k];
+          r |= from & (0xffu << (8 * e));
+        }
+        w[k] = r;
+      }
+      *p = w;
+    }
+  }
+  if (t == 0 && (slot == 0 || grown)) *scale = now;
+}
+
+}  // namespace
+
+extern "C" int pq_kv_append_i8(const void* k, const void* v, int dtype, int64_t k_stride_token, int64_t k_stride_head,
+                               int64_t v_stride_token, int64_t v_stride_head, int8_t* k_cache, int8_t* v_cache,
+                               float* k_scale, float* v_scale, const int32_t* block_table, const int32_t* cu_seqlens,
+                               const int32_t* cached_lens, int64_t batch, int64_t table_width, int64_t tokens,
+                               int64_t heads, int64_t head_dim, int64_t pages, void* stream) {
+  const char* who = "pq_kv_append_i8";
+  PQ_REQUIRE(dtype == PQ_F32 || dtype == PQ_F16 || dtype == PQ_BF16, PQ_ERR_UNSUPPORTED,
+             "%s: dtype code %d (Float, Half or BFloat16)", who, dtype);
+  PQ_REQUIRE(head_dim == 64 || head_dim == 128, PQ_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 64, 128)", who,
+             (long long)head_dim);
+  PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffffLL && table_width >= 0 && table_width <= 0x7fffffffLL / kPage, PQ_ERR_ARG,
+             "%s: batch=%lld table_width=%lld", who, (long long)batch, (long long)table_width);
+  PQ_REQUIRE(tokens >= 0 && tokens <= 0x7fffffffLL && pages >= 0 && pages <= 0x7fffffffLL, PQ_ERR_ARG,
+             "%s: tokens=%lld pages=%lld", who, (long long)tokens, (long long)pages);
+  PQ_REQUIRE(heads >= 1 && heads <= 65535, PQ_ERR_ARG, "%s: heads=%lld (1..65535)", who, (long long)heads);
+  if (batch == 0 || tokens == 0 || table_width == 0 || pages == 0) return PQ_OK;
+  PQ_REQUIRE(k && v && k_cache && v_cache && k_scale && v_scale && block_table && cu_seqlens && cached_lens, PQ_ERR_ARG,
+             "%s: null pointer", who);
+  PQ_REQUIRE(pq::aligned_to(k, 16) && pq::aligned_to(v, 16) && pq::aligned_to(k_cache, 16) && pq::aligned_to(v_cache, 16),
+             PQ_ERR_ARG, "%s: k, v, k_cache and v_cache must be 16-byte aligned", who);
+  const int64_t per = 16 / pq::dtype_size(dtype);
+  PQ_REQUIRE(k_stride_token % per == 0 && k_stride_head % per == 0 && v_stride_token % per == 0 &&
+                 v_stride_head % per == 0, PQ_ERR_ARG, "%s: strides must be multiples of 16 bytes", who);
+  AppendArgs a;
+  a.x[0] = k; a.x[1] = v;
+  a.cache[0] = k_cache; a.cache[1] = v_cache;
+  a.scale[0] = k_scale; a.scale[1] = v_scale;
+  a.st[0] = k_stride_token; a.st[1] = v_stride_token;
+  a.sh[0] = k_stride_head; a.sh[1] = v_stride_head;
+  a.table = block_table; a.cu = cu_seqlens; a.cached = cached_lens;
+  a.batch = static_cast<int>(batch); a.width = static_cast<int>(table_width);
+  a.tokens = static_cast<int>(tokens); a.heads = static_cast<int>(heads); a.pages = static_cast<int>(pages);
+  // pages that n tokens touch: at most n / 64 + 2, and at most n
+  const int64_t most = tokens < tokens / kPage + 2 * batch ? tokens : tokens / kPage + 2 * batch;
+  const dim3 grid(static_cast<unsigned>(most), static_cast<unsigned>(heads), 2);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define PQ_APPEND(DT_)                                                             \
+  if (head_dim == 64) kv_append_kernel<DT_, 64><<<grid, kThreads, 0, s>>>(a);      \
+  else kv_append_kernel<DT_, 128><<<grid, kThreads, 0, s>>>(a);
+  if (dtype == PQ_F32) { PQ_APPEND(PQ_F32) }
+  else if (dtype == PQ_F16) { PQ_APPEND(PQ_F16) }
+  else { PQ_APPEND(PQ_BF16) }
+#undef PQ_APPEND
+  return pq::launch_status("pq_kv_append_i8 launch");
+}

@@ -43,6 +43,10 @@
  *                        (no counterpart)
  *   pq_w4a16_linear_group_fused  the same behind a decoder layer's
  *                        elementwise step (no counterpart)
+ *   pq_attn_*, pq_kv_*   attention between the q/k/v and o linears and its
+ *                        paged int8 cache (no counterpart: the reference
+ *                        calls torch's attention on a bf16 cache,
+ *                        src/alpamayo_r1/utils/system/patches.py:119-141, 489)
  */
 #ifndef PAROQUANT_HIP_H
 #define PAROQUANT_HIP_H
@@ -447,6 +451,84 @@ int pq_w4a8_linear_group_intermediates(const void* x, const void* x2, const void
                                        int count, int64_t m, int64_t k, int krot, unsigned flags, void* workspace,
                                        size_t workspace_bytes, int8_t* codes, float* xscale, int32_t* partials,
                                        void* stream);
+
+/* Causal attention over packed prompts with grouped heads.  q, out:
+ * [tokens_q, kv_heads * group, head_dim], k, v: [tokens_k, kv_heads,
+ * head_dim], of `dtype` (PQ_F16 or PQ_BF16), with strides in values, for a
+ * token and for a head, that are multiples of 8 (out: contiguous); all
+ * 16-byte aligned.  lse: float32 [kv_heads * group, tokens_q].  Sequence b has
+ * query rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 and key rows by
+ * cu_seqlens_k (device memory, batch + 1 entries each; brought into range on
+ * the device).  Query head h reads key/value head h / group.
+ *   out = softmax(scale * q k^T) v,  lse = log(sum exp(scale * q k^T))
+ * causal != 0: query i of n sees keys j <= i + m - n of m.  Rows that see no
+ * key, and rows outside of the sequences, get zeros and lse = -inf; what a
+ * row does not see has no effect on it.  head_dim in {64, 128}; scale > 0. */
+int pq_attn_prompt(const void* q, const void* k, const void* v, int dtype, int64_t q_stride_token,
+                   int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token,
+                   int64_t v_stride_head, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* out,
+                   float* lse, int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t kv_heads, int64_t group,
+                   int64_t head_dim, float scale, int causal, void* stream);
+
+/* The paged int8 cache of the entry points below: k_cache int8 [pages, heads,
+ * 64, head_dim], v_cache int8 [pages, heads, head_dim, 64], k_scale and
+ * v_scale float32 [pages, heads]; a value is code * scale.  Token i of
+ * sequence b is in page block_table[b * table_width + i / 64] (device memory);
+ * a number outside of [0, pages) is no page.  Codes 16-byte aligned. */
+
+/* Puts row i of sequence b (rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of k
+ * and v [tokens, heads, head_dim], any pq_dtype) at place cached_lens[b] + i.
+ * A page's scale is the absmax of what it holds / 127, code = round(x *
+ * (1 / scale)); where new tokens are larger than what their page holds, its
+ * codes become round(code * (old / new)); a page whose first token is new starts
+ * afresh.  NaN counts as 0, infinities saturate and do not count for the
+ * scale; a page whose absmax is below 2^-100 holds zeros.  Tokens whose page
+ * does not exist are dropped.  No page may belong to two sequences of a call. */
+int pq_kv_append_i8(const void* k, const void* v, int dtype, int64_t k_stride_token, int64_t k_stride_head,
+                    int64_t v_stride_token, int64_t v_stride_head, int8_t* k_cache, int8_t* v_cache, float* k_scale,
+                    float* v_scale, const int32_t* block_table, const int32_t* cu_seqlens, const int32_t* cached_lens,
+                    int64_t batch, int64_t table_width, int64_t tokens, int64_t heads, int64_t head_dim, int64_t pages,
+                    void* stream);
+
+/* Bytes of workspace that pq_attn_cache_i8 needs for the partial results of
+ * its workgroups. */
+size_t pq_attn_cache_i8_workspace_size(int64_t batch, int64_t tokens, int64_t group, int64_t head_dim);
+
+/* Attention of each sequence's last tokens over its cache.  q, out [tokens,
+ * kv_heads * group, head_dim] and lse as for pq_attn_prompt; lens[b] (device
+ * memory): tokens of sequence b in the cache, the new ones among them; query
+ * i of n sees tokens j <= i + lens[b] - n.  workspace: 16-byte aligned; its
+ * content does not matter, and calls that may run at the same time must not
+ * share one. */
+int pq_attn_cache_i8(const void* q, int dtype, int64_t q_stride_token, int64_t q_stride_head, const int8_t* k_cache,
+                     const int8_t* v_cache, const float* k_scale, const float* v_scale, const int32_t* block_table,
+                     const int32_t* cu_seqlens, const int32_t* lens, void* out, float* lse, int64_t batch,
+                     int64_t table_width, int64_t tokens, int64_t kv_heads, int64_t group, int64_t head_dim,
+                     int64_t pages, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* weights[b, head, j] += sum over sequence b's rows of the head that see token
+ * j of exp(scale * q . k_j - lse), for j < min(lens[b], span): the softmax
+ * weights of a pq_attn_cache_i8 call, whose lse this takes.  weights: float32
+ * [batch, kv_heads, span].  The order of the sums is fixed. */
+int pq_attn_cache_weights_i8(const void* q, int dtype, int64_t q_stride_token, int64_t q_stride_head,
+                             const int8_t* k_cache, const float* k_scale, const int32_t* block_table,
+                             const int32_t* cu_seqlens, const int32_t* lens, const float* lse, float* weights,
+                             int64_t batch, int64_t table_width, int64_t span, int64_t tokens, int64_t kv_heads,
+                             int64_t group, int64_t head_dim, int64_t pages, float scale, void* stream);
+
+/* Each head of each sequence keeps its last `recent` tokens and, of those
+ * before them, the ones with the largest weights [batch, heads, span], `keep`
+ * in all (equal weights: the earlier token; NaN: lowest).  They move in order
+ * to the front of the pages of new_table [batch, new_width], which no
+ * sequence of the call may be using, rounded to those pages' scales.
+ * weights_out [batch, heads, span]: their weights, zeros behind; lens_out
+ * [batch]: the new lengths; kept int32 [batch, heads, keep]: their old places,
+ * -1 behind.  The output buffers must not overlap the inputs. */
+int pq_kv_evict_i8(int8_t* k_cache, int8_t* v_cache, float* k_scale, float* v_scale, const float* weights,
+                   const int32_t* block_table, const int32_t* lens, const int32_t* new_table, float* weights_out,
+                   int32_t* lens_out, int32_t* kept, int64_t batch, int64_t table_width, int64_t new_width,
+                   int64_t span, int64_t heads, int64_t head_dim, int64_t pages, int64_t keep, int64_t recent,
+                   void* stream);
 
 #ifdef __cplusplus
 }

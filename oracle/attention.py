@@ -1,0 +1,184 @@
+"""Oracle: attention and the paged int8 cache (numpy, CPU).
+
+Attention in float64 from its definition; the cache's scales and codes in float32, operation by operation as their
+definition has them (the GPU's must be equal to the bit):
+
+  scale = absmax / 127 (0 below 2^-100), code = clip(round_half_even(x * (1 / scale)), -127, 127)
+  growth of a page's scale: code' = round_half_even(code * (old / new))
+"""
+
+from __future__ import annotations
+
+import numpy as np
+
+PAGE = 64
+TINY = np.float32(2.0 ** -100)
+
+
+def attend(q, k, v, scale, shift=None):
+    """q [n, d], k, v [m, d] -> (out [n, d], lse [n], sum of p |v| [n, d]) in float64; query i sees keys j <= i + shift
+    (None: all).  Keys that a row does not see take no part, whatever they hold."""
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    n, d = q.shape
+    out, mag, lse = np.zeros((n, d)), np.zeros((n, d)), np.full(n, -np.inf)
+    for i in range(n):
+        m = k.shape[0] if shift is None else min(k.shape[0], max(0, i + shift + 1))
+        if m == 0:
+            continue
+        with np.errstate(invalid="ignore", over="ignore"):
+            s = k[:m] @ q[i] * scale
+            top = s.max()
+            if top == -np.inf:
+                continue
+            p = np.exp(s - top)
+            total = p.sum()
+            lse[i] = top + np.log(total)
+            p = p / total
+            out[i], mag[i] = p @ v[:m], p @ np.abs(v[:m])
+    return out, lse, mag
+
+
+def packed_attention(q, k, v, cu_q, cu_k, scale, causal=True):
+    """q [T, hq, d], k, v [S, hkv, d] -> (out, lse [hq, T], sum of p |v|) over packed sequences."""
+    hq, hkv = q.shape[1], k.shape[1]
+    out, mag = np.zeros(q.shape), np.zeros(q.shape)
+    lse = np.full((hq, q.shape[0]), -np.inf)
+    for b in range(len(cu_q) - 1):
+        a, e, ka, ke = cu_q[b], cu_q[b + 1], cu_k[b], cu_k[b + 1]
+        for h in range(hq):
+            g = h // (hq // hkv)
+            out[a:e, h], lse[h, a:e], mag[a:e, h] = attend(q[a:e, h], k[ka:ke, g], v[ka:ke, g], scale,
+                                                           (ke - ka) - (e - a) if causal else None)
+    return out, lse, mag
+
+
+def page_scale(x):
+    """Scale of values x (float32), from the finite ones."""
+    x = np.asarray(x, np.float32)
+    fine = np.abs(x[np.isfinite(x)])
+    top = fine.max() if fine.size else np.float32(0)
+    return np.float32(0) if top < TINY else np.float32(top / np.float32(127))
+
+
+def encode(x, scale):
+    x = np.asarray(x, np.float32)
+    inv = np.float32(1) / scale if scale > 0 else np.float32(0)
+    with np.errstate(over="ignore", invalid="ignore"):
+        y = np.clip(np.rint(x * inv), -127, 127)
+    return np.where(np.isnan(x), 0, y).astype(np.int8)
+
+
+class Cache:
+    """numpy pools of the cache; V is kept [pages, heads, d, 64]."""
+
+    def __init__(self, k, v, ks, vs):
+        self.k, self.v, self.ks, self.vs = (np.array(x) for x in (k, v, ks, vs))
+
+    def _side(self, side):
+        return (self.k, self.ks) if side == 0 else (self.v.transpose(0, 1, 3, 2), self.vs)
+
+    def append(self, k, v, table, cu, cached):
+        pages, heads = self.ks.shape
+        for side, x in enumerate((k, v)):
+            codes, scales = self._side(side)
+            x = np.asarray(x, np.float32)
+            for b in range(len(cu) - 1):
+                n, held = int(cu[b + 1] - cu[b]), max(int(cached[b]), 0)
+                for j in range(held // PAGE, -(-(held + n) // PAGE)):
+                    if n == 0 or j >= table.shape[1] or not 0 <= table[b, j] < pages:
+                        continue
+                    page = int(table[b, j])
+                    first, last = max(j * PAGE, held), min((j + 1) * PAGE, held + n)
+                    slot = first - j * PAGE
+                    rows = x[cu[b] + first - held:cu[b] + last - held]
+                    for h in range(heads):
+                        fresh = page_scale(rows[:, h])
+                        old = scales[page, h] if slot else np.float32(0)
+                        now = fresh if fresh > old else old
+                        if slot and fresh > old:
+                            ratio = np.float32(old / now)
+                            codes[page, h, :slot] = np.rint(codes[page, h, :slot].astype(np.float32) * ratio).astype(np.int8)
+                        codes[page, h, slot:slot + last - first] = encode(rows[:, h], now)
+                        scales[page, h] = now
+
+    def values(self, side, table_row, length, head, d):
+        """Dequantized [length, d] float64; tokens of pages that do not exist are left out (None in `there`)."""
+        codes, scales = self._side(side)
+        length = min(max(int(length), 0), len(table_row) * PAGE)
+        out, there = np.zeros((length, d)), np.zeros(length, bool)
+        for j in range(-(-length // PAGE)):
+            page, n = int(table_row[j]), min(PAGE, length - j * PAGE)
+            if 0 <= page < codes.shape[0]:
+                out[j * PAGE:j * PAGE + n] = codes[page, head, :n].astype(np.float64) * np.float64(scales[page, head])
+                there[j * PAGE:j * PAGE + n] = True
+        return out, there
+
+    def attention(self, q, table, cu, lens, scale):
+        """(out, lse, sum of p |v|, sum of |v|) of the last tokens over the cache."""
+        heads = self.ks.shape[1]
+        hq, d = q.shape[1:]
+        out, mag, lse = np.zeros(q.shape), np.zeros(q.shape), np.full((hq, q.shape[0]), -np.inf)
+        for b in range(len(cu) - 1):
+            n = int(cu[b + 1] - cu[b])
+            for h in range(hq):
+                g = h // (hq // heads)
+                k, there = self.values(0, table[b], lens[b], g, d)
+                v, _ = self.values(1, table[b], lens[b], g, d)
+                for i in range(n):
+                    sees = there[:max(0, len(k) - n + i + 1)]
+                    idx = np.nonzero(sees)[0]
+                    o, z, a = attend(q[cu[b] + i:cu[b] + i + 1, h], k[idx], v[idx], scale)
+                    out[cu[b] + i, h], lse[h, cu[b] + i], mag[cu[b] + i, h] = o[0], z[0], a[0]
+        return out, lse, mag
+
+    def weights(self, q, table, cu, lens, lse, scale, span):
+        heads = self.ks.shape[1]
+        hq, d = q.shape[1:]
+        w = np.zeros((len(cu) - 1, heads, span))
+        for b in range(len(cu) - 1):
+            n = int(cu[b + 1] - cu[b])
+            for h in range(hq):
+                g = h // (hq // heads)
+                k, there = self.values(0, table[b], lens[b], g, d)
+                for i in range(n):
+                    m = max(0, len(k) - n + i + 1)
+                    z = float(lse[h, cu[b] + i])
+                    if m == 0 or z == -np.inf:
+                        continue
+                    p = np.exp(k[:m] @ np.asarray(q[cu[b] + i, h], np.float64) * scale - z) * there[:m]
+                    w[b, g, :min(m, span)] += p[:span]
+        return w
+
+    def evict(self, weights, table, lens, new_table, keep, recent):
+        """(weights, lens, kept); the pools are changed in place."""
+        batch, heads, span = weights.shape
+        pages = self.ks.shape[0]
+        out, kept = np.zeros_like(weights), np.full((batch, heads, keep), -1, np.int32)
+        left_all = np.zeros(batch, np.int32)
+        for b in range(batch):
+            n = min(max(int(lens[b]), 0), table.shape[1] * PAGE, span)
+            fixed = max(0, n - recent)
+            left_all[b] = min(n, keep)
+            for h in range(heads):
+                w = weights[b, h, :n]
+                rank = np.where(np.isnan(w[:fixed]), -np.inf, w[:fixed])
+                nan = np.isnan(w[:fixed])
+                order = np.lexsort((np.arange(fixed), nan, -rank))   # largest first; NaN behind -inf; the earlier of equals
+                at = np.sort(np.concatenate([order[:min(n, keep) - (n - fixed)], np.arange(fixed, n)])).astype(int)
+                kept[b, h, :len(at)], out[b, h, :len(at)] = at, w[at]
+                for side in (0, 1):
+                    codes, scales = self._side(side)
+                    for j in range(-(-len(at) // PAGE)):
+                        page = int(new_table[b, j])
+                        if not 0 <= page < pages:
+                            continue
+                        rows = []
+                        for pos in at[j * PAGE:(j + 1) * PAGE]:
+                            src = int(table[b, pos // PAGE])
+                            ok = 0 <= src < pages
+                            rows.append(codes[src, h, pos % PAGE].astype(np.float32) * scales[src, h] if ok else
+                                        np.zeros(codes.shape[3], np.float32))
+                        rows = np.stack(rows)
+                        scales[page, h] = page_scale(rows)
+                        codes[page, h, :len(rows)] = encode(rows, scales[page, h])
+        return out, left_all, kept
