@@ -65,6 +65,31 @@ __device__ __forceinline__ Span span_of(const int* cu, int b, int total) {
 
 struct Found { int b; int64_t local; };   // b < 0: past the last one
 
+// x of the lanes that the DPP control takes it from, 0 where there is none.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int64_t dpp_or_0(int64_t x) {
+  const u2 w = __builtin_bit_cast(u2, x);
+  const u2 r = {static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w[0]), CTRL, ROW_MASK, 0xf, false)),
+                static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(w[1]), CTRL, ROW_MASK, 0xf, false))};
+  return __builtin_bit_cast(int64_t, r);
+}
+// Sums over the lanes up to each: four shifts within rows of 16, then the rows' last lanes.
+__device__ __forceinline__ int64_t wave_scan(int64_t x) {
+  x += dpp_or_0<0x111, 0xf>(x);   // row_shr:1
+  x += dpp_or_0<0x112, 0xf>(x);
+  x += dpp_or_0<0x114, 0xf>(x);
+  x += dpp_or_0<0x118, 0xf>(x);
+  x += dpp_or_0<0x142, 0xa>(x);   // row_bcast:15
+  x += dpp_or_0<0x143, 0xc>(x);   // row_bcast:31
+  return x;
+}
+__device__ __forceinline__ int64_t read_lane(int64_t x, int lane) {
+  const u2 w = __builtin_bit_cast(u2, x);
+  const u2 r = {static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(w[0]), lane)),
+                static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(w[1]), lane))};
+  return __builtin_bit_cast(int64_t, r);
+}
+
 // The sequence in which number idx of the numbers cost(0) + cost(1) + ... lies, by all lanes of a wave: each takes one
 // sequence of 64 at a time.
 template <class F>
@@ -74,18 +99,13 @@ __device__ __forceinline__ Found find_seq(int batch, int64_t idx, F cost) {
   for (int base = 0; base < batch; base += 64) {
     const int b = base + lane;
     const int64_t own = b < batch ? cost(b) : 0;
-    int64_t incl = own;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const int64_t up = __shfl_up(incl, s);
-      if (lane >= s) incl += up;
-    }
+    const int64_t incl = wave_scan(own);
     const uint64_t past = __ballot(idx < before + incl);
     if (past) {
       const int at = __builtin_ctzll(past);
-      return {base + at, idx - before - __shfl(incl - own, at)};
+      return {base + at, idx - before - read_lane(incl - own, at)};
     }
-    before += __shfl(incl, 63);
+    before += read_lane(incl, 63);
   }
   return {-1, idx - before};
 }
@@ -94,9 +114,7 @@ template <class F>
 __device__ __forceinline__ int64_t sum_seqs(int batch, F cost) {
   int64_t sum = 0;
   for (int b = lane_id(); b < batch; b += 64) sum += cost(b);
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
-  return sum;
+  return read_lane(wave_scan(sum), 63);
 }
 
 // ---------------------------------------------------------------------------

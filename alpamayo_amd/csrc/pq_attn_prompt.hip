@@ -17,6 +17,7 @@
 // p is rounded to the inputs' type (half a step 2^-9 of the value in bf16,
 // 2^-12 in fp16, as the outputs are); scores, sums and statistics are float32.
 #include <algorithm>
+#include <type_traits>
 
 #include "pq_attn.h"
 #include "pq_device.h"
@@ -73,24 +74,37 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// Copies kKeys rows from row k0 on (past the last: the last again) to LDS, swizzled.
+// The 16-byte chunks of kKeys rows that a thread copies to LDS: byte offsets from the first row.  Rows past `last` are
+// taken from it.
 template <int D>
-__device__ __forceinline__ void stage(const uint16_t* base, int64_t stride, int k0, int last, uint16_t* lds) {
-  constexpr int kChunks = D / 8, kEach = kKeys * kChunks / kThreads;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id();
+struct Chunks {
+  static constexpr int kRow = D / 8, kEach = kKeys * kRow / kThreads;
+  uint32_t off[kEach];
+  __device__ __forceinline__ Chunks(int64_t stride, int last) {
+    const int wave = threadIdx.x >> 6, lane = lane_id();
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int at = (wave * kEach + i) * 64, c = (at + lane) % kChunks, r = (at + lane) / kChunks;
-    const uint16_t* src = base + static_cast<int64_t>(min(k0 + r, last)) * stride + (c ^ swz<D>(r)) * 8;
-    pqd::lds_copy16(src, pqd::lds_addr(lds) + at * 16);
+    for (int i = 0; i < kEach; ++i) {
+      const int at = (wave * kEach + i) * 64 + lane, c = at % kRow, r = at / kRow;
+      off[i] = static_cast<uint32_t>(min(r, last)) * static_cast<uint32_t>(2 * stride) + (c ^ swz<D>(r)) * 16;
+    }
   }
-}
+  // base: the first row's address, the same in every lane
+  __device__ __forceinline__ void copy(const uint16_t* base, const uint16_t* lds) const {
+    const uint32_t to = pqd::lds_addr(lds) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (kEach * 1024);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + i * 1024), "v"(off[i]),
+                   "s"(base)
+                   : "memory", "m0");
+  }
+};
 
 template <int D, bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) {
   constexpr int kDt = D / 32, kSteps = D / 16;
-  __shared__ __align__(16) uint16_t ks[kKeys * D], vs[kKeys * D];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, col = lane & 31;
+  __shared__ __align__(16) uint16_t lds[2][2][kKeys * D];   // two stages of keys and values
+  const int t = threadIdx.x, lane = t & 63, half = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int head = blockIdx.x % a.heads;
   const int idx = a.tiles - 1 - blockIdx.x / a.heads;   // late rows of a prompt see most keys: they start first
 
@@ -148,81 +162,101 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
   // V: the lane's address in a transposing read of 4 keys by 16 channels
   const int l16 = lane & 15, vsub = lane >> 4 & 1;
 
-  for (int k0 = 0; k0 < end; k0 += kKeys) {
-    stage<D>(kb, a.k_st, k0, sk.count - 1, ks);
-    stage<D>(vb, a.v_st, k0, sk.count - 1, vs);
-    pqd::wait_vmcnt<0>();
-    __syncthreads();
-    if (k0 < wend) {
-      f16v s[2];
+  // the last tile's rows end with the sequence
+  const int64_t kstep = kKeys * a.k_st, vstep = kKeys * a.v_st;
+  const Chunks<D> kc(a.k_st, kKeys), vc(a.v_st, kKeys);
+  const auto stage = [&](int k0, int to) {
+    const int tile = k0 / kKeys;
+    if (k0 + kKeys <= sk.count) {
+      kc.copy(kb + tile * kstep, lds[to][0]);
+      vc.copy(vb + tile * vstep, lds[to][1]);
+    } else {
+      const Chunks<D> kl(a.k_st, sk.count - 1 - k0), vl(a.v_st, sk.count - 1 - k0);
+      kl.copy(kb + tile * kstep, lds[to][0]);
+      vl.copy(vb + tile * vstep, lds[to][1]);
+    }
+  };
+
+  // One tile of keys.  MASKED: some rows of the wave do not see some of its keys.
+  const auto tile = [&](auto mask, int k0, const uint16_t* ks, const uint16_t* vs) {
+    constexpr bool kMasked = decltype(mask)::value;
+    f16v s[2] = {f16v{}, f16v{}};
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        s[u] = f16v{};
         const int r = 32 * u + kr;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-          s[u] = mfma32<BF16>(*reinterpret_cast<const s8*>(ks + r * D + ((2 * i + half) ^ swz<D>(r)) * 8), qf[i], s[u]);
+        s[u] = mfma32<BF16>(*reinterpret_cast<const s8*>(ks + r * D + ((2 * i + half) ^ swz<D>(r)) * 8), qf[i], s[u]);
       }
-      const bool masked = k0 + kKeys > sure;
-      float big = -INFINITY;
+    float big = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (masked && k0 + 32 * u + 16 * (i >> 3) + 8 * half + (i & 7) >= limit) s[u][i] = -INFINITY;
-          big = fmaxf(big, s[u][i]);
-        }
-      big = fmaxf(m, max_xor32(big) * c);
-      const float base = big == -INFINITY ? 0.0f : big;
-      const float alpha = exp2_fast(m - base);
-      m = big;
-      float sum = 0.0f;
-      s8 pf[4];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float x = exp2_fast(__builtin_fmaf(s[u][i], c, -base)), y = exp2_fast(__builtin_fmaf(s[u][i + 1], c, -base));
-          sum += x + y;
-          const uint32_t w = pack2<BF16>(x, y);
-          pf[2 * u + (i >> 3)][i & 7] = static_cast<short>(w & 0xffffu);
-          pf[2 * u + (i >> 3)][(i & 7) + 1] = static_cast<short>(w >> 16);
-        }
-      l = l * alpha + sum;
+      for (int i = 0; i < 16; ++i) {
+        if constexpr (kMasked)
+          if (k0 + 32 * u + 16 * (i >> 3) + 8 * half + (i & 7) >= limit) s[u][i] = -INFINITY;
+        big = fmaxf(big, s[u][i]);
+      }
+    // A row's maximum moves only by more than 8 (in base 2) at a time: p then stays below 256, and most tiles need no
+    // rescaling.  Each row goes by itself, so that no row's bits depend on what its neighbours hold.
+    big = max_xor32(big) * c;
+    const bool moves = big > m + 8.0f;
+    if (__any(moves)) {
+      const float now = moves ? big : m;
+      const float alpha = moves ? exp2_fast(m - now) : 1.0f;
+      m = now;
+      l *= alpha;
 #pragma unroll
       for (int i = 0; i < kDt; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+    s8 pf[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      u4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = exp2_fast(__builtin_fmaf(s[u >> 1][8 * (u & 1) + 2 * i], c, -base));
+        const float y = exp2_fast(__builtin_fmaf(s[u >> 1][8 * (u & 1) + 2 * i + 1], c, -base));
+        sum += x + y;
+        w[i] = pack2<BF16>(x, y);
+      }
+      pf[u] = __builtin_bit_cast(s8, w);
+    }
+    l += sum;
 
-      // In a masked tile a value that is not finite must not meet the weight 0 of a row that does not see its key:
-      // there it takes no part in the product and is added to the rows that do see it.
-      bool odd = false;
+    // In a masked tile a value that is not finite must not meet the weight 0 of a row that does not see its key:
+    // there it takes no part in the product and is added to the rows that do see it.
+    uint32_t odd = 0;
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int i = 0; i < kDt; ++i) {
-          s8 vf;
+      for (int i = 0; i < kDt; ++i) {
+        u2 w[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int r = 16 * u + 8 * half + 4 * x + (l16 >> 2);
-            const int ch = (4 * i + 2 * vsub + (l16 >> 1 & 1)) ^ swz<D>(r);
-            const s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s4*)(vs + r * D + ch * 8 + (l16 & 1) * 4));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vf[4 * x + e] = w[e];
-          }
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              constexpr int kInf = BF16 ? 0x7f80 : 0x7c00;
-              const bool bad = (vf[e] & kInf) == kInf;
-              odd |= bad;
-              vf[e] = bad ? static_cast<short>(0) : vf[e];
-            }
-          }
-          o[i] = mfma32<BF16>(vf, pf[u], o[i]);
+        for (int x = 0; x < 2; ++x) {
+          const int r = 16 * u + 8 * half + 4 * x + (l16 >> 2);
+          const int ch = (4 * i + 2 * vsub + (l16 >> 1 & 1)) ^ swz<D>(r);
+          w[x] = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                            (__attribute__((address_space(3))) s4*)(vs + r * D + ch * 8 + (l16 & 1) * 4)));
         }
-      if (masked && __ballot(odd)) {
+        u4 vf = {w[0][0], w[0][1], w[1][0], w[1][1]};
+        if constexpr (kMasked) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
+            const uint32_t bad = ((vf[e] & kInf) == kInf ? 0xffffu : 0) | ((vf[e] >> 16 & kInf) == kInf ? 0xffff0000u : 0);
+            odd |= bad;
+            vf[e] &= ~bad;
+          }
+        }
+        o[i] = mfma32<BF16>(__builtin_bit_cast(s8, vf), pf[u], o[i]);
+      }
+    if constexpr (kMasked) {
+      if (__any(odd != 0)) {
         for (int key = 0; key < kKeys && k0 + key < sk.count; ++key) {
           if (k0 + key >= limit) continue;
 #pragma unroll
@@ -236,7 +270,17 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
         }
       }
     }
+  };
+
+  if (end > 0) stage(0, 0);
+  for (int k0 = 0; k0 < end; k0 += kKeys) {
+    // this stage's copies are done, and no wave reads the other one any more: the next tile's go there
+    pqd::wait_vmcnt<0>();
     __syncthreads();
+    const int at = k0 / kKeys & 1;
+    if (k0 + kKeys < end) stage(k0 + kKeys, at ^ 1);
+    if (k0 + kKeys <= sure) tile(std::false_type{}, k0, lds[at][0], lds[at][1]);
+    else if (k0 < wend) tile(std::true_type{}, k0, lds[at][0], lds[at][1]);
   }
 
   l = sum_xor32(l);
@@ -279,6 +323,10 @@ extern "C" int pq_attn_prompt(const void* q, const void* k, const void* v, int d
   PQ_REQUIRE(q_stride_token % 8 == 0 && q_stride_head % 8 == 0 && k_stride_token % 8 == 0 && k_stride_head % 8 == 0 &&
                  v_stride_token % 8 == 0 && v_stride_head % 8 == 0, PQ_ERR_ARG,
              "%s: strides must be multiples of 8 values", who);
+  // a tile's rows are addressed by 32-bit offsets from its first
+  PQ_REQUIRE(k_stride_token >= 0 && k_stride_token <= 1 << 24 && v_stride_token >= 0 && v_stride_token <= 1 << 24, PQ_ERR_ARG,
+             "%s: k_stride_token=%lld v_stride_token=%lld (0..2^24)", who, (long long)k_stride_token,
+             (long long)v_stride_token);
   PromptArgs a;
   a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
   a.out = static_cast<uint16_t*>(out); a.lse = lse; a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k;
