@@ -26,6 +26,13 @@ __device__ __forceinline__ int lane_id() { return static_cast<int>(threadIdx.x &
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
+// A read through the scalar cache, of memory that no part of the running kernel writes, at an address that is the same
+// in every lane: it does not queue behind the vector loads in flight.
+template <class T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(p));
+}
+
 // The other half of the wave's value combined with the own: every lane ends with both.
 __device__ __forceinline__ float max_xor32(float x) {
   const u2 r = __builtin_bit_cast(

@@ -29,6 +29,7 @@
 #include <algorithm>
 
 #include "pq_attn.h"
+#include "pq_device.h"
 
 namespace {
 
@@ -37,6 +38,10 @@ using namespace pqa;
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kWorkers = 512;
+#ifndef KRT
+#define KRT 1
+#endif
+constexpr int kRT = KRT;
 
 struct CacheArgs {
   const void* q;                      // [tokens, heads * group, d]
@@ -138,14 +143,16 @@ __device__ __forceinline__ void load_k(const int8_t* page, u4 (&kr)[4][D / 64]) 
   }
 }
 
-template <int D, int RT, bool BF16>
-__global__ __launch_bounds__(kThreads) void attn_cache_kernel(CacheArgs a) {
-  constexpr int kRows = 16 * RT, kDt = D / 16;
+// RT row tiles of 16 for each wave, RW waves with rows of their own on the same pages.
+template <int D, int RT, int RW, bool BF16>
+__global__ __launch_bounds__(kThreads, RT == 4 ? 1 : 2) void attn_cache_kernel(CacheArgs a) {
+  constexpr int kRows = 16 * RT * RW, kDt = D / 16, kStreams = kWaves / RW;
   constexpr int kPitch = D + 4;
   __shared__ __align__(16) float so[kWaves][16][kPitch];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
   using P = Plan<kRows>;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, g = lane >> 4, col = lane & 15;
+  const int t = threadIdx.x, lane = t & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), stream = wave / RW, part_of = wave % RW;
 
   const auto cost = [&](int b) { return P::cost(a, b); };
   const int64_t total = sum_seqs(a.batch, cost);
@@ -168,10 +175,11 @@ __global__ __launch_bounds__(kThreads) void attn_cache_kernel(CacheArgs a) {
     int limit[RT];     // keys that the lane's row sees
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      load_q<D, BF16>(a, sp.first, rows, head, row0 + 16 * i, qf[i], mult[i]);
-      limit[i] = min((row0 + 16 * i + col) / a.group + len - sp.count + 1, len);
+      const int first = row0 + 16 * (RT * part_of + i);
+      load_q<D, BF16>(a, sp.first, rows, head, first, qf[i], mult[i]);
+      limit[i] = min((first + col) / a.group + len - sp.count + 1, len);
     }
-    const int sure = row0 / a.group + len - sp.count + 1;   // keys that every row sees
+    const int sure = (row0 + 16 * RT * part_of) / a.group + len - sp.count + 1;   // keys that every row of the wave sees
 
     float m[RT], l[RT];
     f4 o[RT][kDt];
@@ -183,63 +191,84 @@ __global__ __launch_bounds__(kThreads) void attn_cache_kernel(CacheArgs a) {
       for (int k = 0; k < kDt; ++k) o[i][k] = f4{0, 0, 0, 0};
     }
 
-    for (int p = p0 + wave; p < p1; p += kWaves) {
-      const int page = a.table[static_cast<int64_t>(f.b) * a.width + p];
-      if (page < 0 || page >= a.pages) continue;
-      const int64_t ph = static_cast<int64_t>(page) * a.heads + head;
-      const int8_t* kp = a.kc + ph * (kPage * D);
+    // The next page's codes are asked for as soon as the registers of this one's are free: K behind the first product,
+    // V behind the second; its number one page ahead of that.
+    const int* table = a.table + static_cast<int64_t>(f.b) * a.width;
+    u4 kr[4][D / 64], vr[kDt];
+    float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    const auto load_v = [&](int64_t ph) {
       const int8_t* vp = a.vc + ph * (kPage * D);
-      u4 kr[4][D / 64], vr[kDt];
-      load_k<D, true>(kp, kr);
 #pragma unroll
       for (int k = 0; k < kDt; ++k) vr[k] = *reinterpret_cast<const u4*>(vp + (16 * k + col) * kPage + g * 16);
-      const float ks = a.ks[ph], vs = a.vs[ph];
+    };
+    const auto number = [&](int p) { return scalar_load(table + p); };
+    // page and head of place p; a number that is no page: page 0, with no token to see
+    const auto page_head = [&](int id) { return static_cast<int64_t>(id < 0 || id >= a.pages ? 0 : id) * a.heads + head; };
 
+    // seen: tokens of the cache that rows may see; masked: some row does not see some token of the page
+    const auto step = [&](bool masked, int seen, int p, int64_t ph_next) {
+      ks_next = scalar_load(a.ks + ph_next);
+      vs_next = scalar_load(a.vs + ph_next);
       f4 s[RT][4];
 #pragma unroll
       for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) s[i][q] = f4{0, 0, 0, 0};
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int k = 0; k < D / 32; ++k)
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
+        for (int q = 0; q < 4; ++q) {
           const h8 kf = codes_f16(kr[q][k >> 1][2 * (k & 1)], kr[q][k >> 1][2 * (k & 1) + 1]);
 #pragma unroll
           for (int i = 0; i < RT; ++i) s[i][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i][k], s[i][q], 0, 0, 0);
         }
+      load_k<D, true>(a.kc + ph_next * (kPage * D), kr);
+      __builtin_amdgcn_sched_barrier(0);
 
       // the lane's tokens: 16 g + 4 q + e
-      const bool masked = (p + 1) * kPage > sure;
       h8 pf[RT][2];
-      float alpha[RT];
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        const float c = ks * mult[i];
+        // never 0: what is masked stays -inf, and scores of rows and pages of zeros stay as good as 0
+        const float c = fmaxf(ks * mult[i], 1e-37f);
         float big = -INFINITY;
+        if (masked) {
+          const int see = min(limit[i], seen) - p * kPage - 16 * g;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][q][e] = 4 * q + e >= see ? -INFINITY : s[i][q][e];
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = s[i][q][e] * c;
-            if (masked && p * kPage + 16 * g + 4 * q + e >= limit[i]) x = -INFINITY;
-            s[i][q][e] = x;
-            big = fmaxf(big, x);
-          }
-        big = fmaxf(m[i], max_xor32(max_xor16(big)));
-        const float base = big == -INFINITY ? 0.0f : big;
-        alpha[i] = exp2_fast(m[i] - base);
-        m[i] = big;
+          for (int e = 0; e < 4; ++e) big = fmaxf(big, s[i][q][e]);
+        // a row's maximum moves by more than 8 (in base 2) at a time, each row by itself
+        big = max_xor32(max_xor16(big)) * c;
+        const bool moves = big > m[i] + 8.0f;
+        if (__any(moves)) {
+          const float now = moves ? big : m[i];
+          const float alpha = moves ? exp2_fast(m[i] - now) : 1.0f;
+          m[i] = now;
+          l[i] *= alpha;
+#pragma unroll
+          for (int k = 0; k < kDt; ++k) o[i][k] *= alpha;
+        }
+        const float base = m[i] == -INFINITY ? 0.0f : m[i];
         float sum = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 2; ++q) {
+          u4 w;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = exp2_fast(s[i][q][e] - base);
-            sum += x;
-            pf[i][q >> 1][4 * (q & 1) + e] = static_cast<_Float16>(x);
+            const float x = exp2_fast(__builtin_fmaf(s[i][2 * q + (e >> 1)][2 * (e & 1)], c, -base));
+            const float y = exp2_fast(__builtin_fmaf(s[i][2 * q + (e >> 1)][2 * (e & 1) + 1], c, -base));
+            sum += x + y;
+            w[e] = pqd::pk_f16(x, y);
           }
-        l[i] = l[i] * alpha[i] + sum;
+          pf[i][q] = __builtin_bit_cast(h8, w);
+        }
+        l[i] += sum;
       }
 #pragma unroll
       for (int k = 0; k < kDt; ++k) {
@@ -250,12 +279,36 @@ __global__ __launch_bounds__(kThreads) void attn_cache_kernel(CacheArgs a) {
           x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[i][0], x, 0, 0, 0);
           x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[i][1], x, 0, 0, 0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][k][e] = __builtin_fmaf(x[e], vs, o[i][k][e] * alpha[i]);
+          for (int e = 0; e < 4; ++e) o[i][k][e] = __builtin_fmaf(x[e], vs, o[i][k][e]);
         }
+      }
+      load_v(ph_next);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+
+    int p = p0 + stream;
+    if (p < p1) {
+      int id = number(p), id_next = p + kStreams < p1 ? number(p + kStreams) : 0;
+      const int64_t ph = page_head(id);
+      ks = scalar_load(a.ks + ph);
+      vs = scalar_load(a.vs + ph);
+      load_k<D, true>(a.kc + ph * (kPage * D), kr);
+      __builtin_amdgcn_sched_barrier(0);   // K before V, as in the loop: the wait for K then leaves V in flight
+      load_v(ph);
+      __builtin_amdgcn_sched_barrier(0);
+      for (; p < p1; p += kStreams) {
+        // behind the last page the loads, which the waits count on, go to that page again
+        const bool there = id >= 0 && id < a.pages;
+        id = p + kStreams < p1 ? id_next : id;
+        const int64_t ph_next = page_head(id);
+        if (p + 2 * kStreams < p1) id_next = number(p + 2 * kStreams);
+        step(!there || (p + 1) * kPage > sure, there ? len : 0, p, ph_next);
+        ks = ks_next;
+        vs = vs_next;
       }
     }
 
-    // the four waves' results of the segment
+    // the results of the segment, from the waves that went through its pages
     const bool whole = p0 == 0 && p1 == npages;
     float* part = a.part + (2 * w + (at == from ? 0 : 1)) * part_floats<kRows, D>();
 #pragma unroll
@@ -268,22 +321,24 @@ __global__ __launch_bounds__(kThreads) void attn_cache_kernel(CacheArgs a) {
 #pragma unroll
       for (int k = 0; k < kDt; ++k) *reinterpret_cast<f4*>(&so[wave][col][16 * k + 4 * g]) = o[i][k];
       __syncthreads();
-      const int r = t >> 4, row = row0 + 16 * i + r;
-      if (row < rows) {
-        float big = sm[0][r];
 #pragma unroll
-        for (int q = 1; q < kWaves; ++q) big = fmaxf(big, sm[q][r]);
+      for (int x = 0; x < RW; ++x) {
+        const int r = t >> 4, local = 16 * (RT * x + i) + r, row = row0 + local;
+        if (row >= rows) continue;
+        float big = sm[x][r];
+#pragma unroll
+        for (int q = 1; q < kStreams; ++q) big = fmaxf(big, sm[RW * q + x][r]);
         const float base = big == -INFINITY ? 0.0f : big;
         float sum = 0.0f;
         f4 acc[D / 64];
 #pragma unroll
         for (int k = 0; k < D / 64; ++k) acc[k] = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int q = 0; q < kWaves; ++q) {
-          const float x = exp2_fast(sm[q][r] - base);
-          sum += sl[q][r] * x;
+        for (int q = 0; q < kStreams; ++q) {
+          const float y = exp2_fast(sm[RW * q + x][r] - base);
+          sum += sl[RW * q + x][r] * y;
 #pragma unroll
-          for (int k = 0; k < D / 64; ++k) acc[k] += *reinterpret_cast<const f4*>(&so[q][r][64 * k + 4 * (t & 15)]) * x;
+          for (int k = 0; k < D / 64; ++k) acc[k] += *reinterpret_cast<const f4*>(&so[RW * q + x][r][64 * k + 4 * (t & 15)]) * y;
         }
         if (whole) {
           const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
@@ -300,11 +355,10 @@ __global__ __launch_bounds__(kThreads) void attn_cache_kernel(CacheArgs a) {
           if ((t & 15) == 0) a.lse[static_cast<int64_t>(h) * a.tokens + token] = (big + log2_fast(sum)) * kLn2;
         } else {
 #pragma unroll
-          for (int k = 0; k < D / 64; ++k)
-            *reinterpret_cast<f4*>(part + (16 * i + r) * D + 64 * k + 4 * (t & 15)) = acc[k];
+          for (int k = 0; k < D / 64; ++k) *reinterpret_cast<f4*>(part + local * D + 64 * k + 4 * (t & 15)) = acc[k];
           if ((t & 15) == 0) {
-            part[kRows * D + 16 * i + r] = big;
-            part[kRows * D + kRows + 16 * i + r] = sum;
+            part[kRows * D + local] = big;
+            part[kRows * D + kRows + local] = sum;
           }
         }
       }
@@ -314,19 +368,19 @@ __global__ __launch_bounds__(kThreads) void attn_cache_kernel(CacheArgs a) {
   }
 }
 
-// Joins the partial results of a row whose unit spans workgroups.  One workgroup per (query head, token): its waves
-// take the parts in turn.  Rows outside of the sequences and rows of empty ones get zeros and lse = -inf.
+// Joins the partial results of the rows whose unit spans workgroups.  A workgroup takes four (query head, token) rows of a
+// token: a wave each, or, where the parts are many, its waves together on one row after the other.  Rows outside of the
+// sequences and rows of empty ones get zeros and lse = -inf.
 template <int D, int RT, bool BF16>
 __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) {
   constexpr int kRows = 16 * RT, kV = D / 64;
   __shared__ float so[kWaves][D], sl[kWaves], sm[kWaves];
   using P = Plan<kRows>;
-  const int token = blockIdx.x, h = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int head = h / a.group;
-  uint16_t* op = static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(token) * a.heads * a.group + h) * D;
-  float* lse = a.lse + static_cast<int64_t>(h) * a.tokens + token;
+  const int token = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int hq = a.heads * a.group;
 
-  // the sequence that the row belongs to, and the pages of the units before it
+  // the sequence that the token belongs to, and the pages of the units before it
   const auto cost = [&](int b) { return P::cost(a, b); };
   int b = -1;
   int64_t before = 0, total = 0;
@@ -336,72 +390,126 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
     const Span sp = there ? span_of(a.cu, own, a.tokens) : Span{0, 0};
     const int64_t c = there ? cost(own) : 0;
     const uint64_t hit = __ballot(token >= sp.first && token < sp.first + sp.count);
-    int64_t sum = c, part = hit && lane < __builtin_ctzll(hit) ? c : 0;
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) {
-      sum += __shfl_xor(sum, s);
-      part += __shfl_xor(part, s);
-    }
+    const int64_t incl = wave_scan(c);
     if (b < 0 && hit) {
-      b = base + __builtin_ctzll(hit);
-      before = total + part;
+      const int at = __builtin_ctzll(hit);
+      b = base + at;
+      before = total + read_lane(incl - c, at);
     }
-    total += sum;
+    total += read_lane(incl, 63);
   }
   const int len = b < 0 ? 0 : seq_len(a, b);
+  const auto out_row = [&](int h) { return static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(token) * hq + h) * D; };
+  const auto lse_of = [&](int h) { return a.lse + static_cast<int64_t>(h) * a.tokens + token; };
   if (len == 0) {
-    for (int i = t; i < D; i += kThreads) op[i] = 0;
-    if (t == 0) *lse = -INFINITY;
+    const int h = blockIdx.y * kWaves + wave;
+    if (h < hq) {
+#pragma unroll
+      for (int k = 0; k < kV; ++k) out_row(h)[lane * kV + k] = 0;
+      if (lane == 0) *lse_of(h) = -INFINITY;
+    }
     return;
   }
   const Span sp = span_of(a.cu, b, a.tokens);
   const int npages = (len + kPage - 1) / kPage;
-  const int row = (token - sp.first) * a.group + h - head * a.group;
-  const int64_t begin = before + (static_cast<int64_t>(row / kRows) * a.heads + head) * npages, end = begin + npages;
   const int64_t n = P::workers(a, total);
-  const int64_t w0 = P::owner(begin, total, n), w1 = P::owner(end - 1, total, n);
-  if (w0 == w1) return;   // written by the workgroup that had all of it
 
-  const int r = row % kRows;
-  const auto part = [&](int64_t w) {
-    const bool first = w > w0 || P::begin(w, total, n) == begin;
-    return a.part + (2 * w + (first ? 0 : 1)) * part_floats<kRows, D>();
+  // parts w0 + first, w0 + first + step, ... of a row into m, l, o
+  struct Parts { int64_t begin, w0, w1; int r; };
+  const auto parts_of = [&](int h) {
+    const int head = h / a.group, row = (token - sp.first) * a.group + h - head * a.group;
+    Parts q;
+    q.begin = before + (static_cast<int64_t>(row / kRows) * a.heads + head) * npages;
+    q.w0 = P::owner(q.begin, total, n);
+    q.w1 = P::owner(q.begin + npages - 1, total, n);
+    q.r = row % kRows;
+    return q;
   };
-  float m = -INFINITY, l = 0.0f, o[kV];
+  const auto gather = [&](const Parts& q, int first, int step, float& m, float& l, float (&o)[kV]) {
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kV; ++k) o[k] = 0.0f;
-  for (int64_t w = w0 + wave; w <= w1; w += kWaves) {
-    const float* p = part(w);
-    const float pm = p[kRows * D + r], pl = p[kRows * D + kRows + r];
-    const float big = fmaxf(m, pm), base = big == -INFINITY ? 0.0f : big;
-    const float ca = exp2_fast(m - base), cb = exp2_fast(pm - base);
-    l = l * ca + pl * cb;
+    for (int k = 0; k < kV; ++k) o[k] = 0.0f;
+    constexpr int kAhead = 4;
+    for (int64_t w = q.w0 + first; w <= q.w1; w += kAhead * step) {
+      float pm[kAhead], pl[kAhead], po[kAhead][kV];
 #pragma unroll
-    for (int k = 0; k < kV; ++k) o[k] = o[k] * ca + p[r * D + lane * kV + k] * cb;
-    m = big;
-  }
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
-  }
+      for (int i = 0; i < kAhead; ++i) {
+        pm[i] = -INFINITY;
+        pl[i] = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kV; ++k) so[wave][lane * kV + k] = o[k];
-  __syncthreads();
-  if (t < D) {
-    float big = sm[0];
+        for (int k = 0; k < kV; ++k) po[i][k] = 0.0f;
+        const int64_t x = w + i * step;
+        if (x <= q.w1) {
+          const bool own = x > q.w0 || P::begin(x, total, n) == q.begin;
+          const float* p = a.part + (2 * x + (own ? 0 : 1)) * part_floats<kRows, D>();
+          pm[i] = p[kRows * D + q.r];
+          pl[i] = p[kRows * D + kRows + q.r];
 #pragma unroll
-    for (int q = 1; q < kWaves; ++q) big = fmaxf(big, sm[q]);
-    const float base = big == -INFINITY ? 0.0f : big;
-    float sum = 0.0f, acc = 0.0f;
+          for (int k = 0; k < kV; ++k) po[i][k] = p[q.r * D + lane * kV + k];
+        }
+      }
 #pragma unroll
-    for (int q = 0; q < kWaves; ++q) {
-      const float x = exp2_fast(sm[q] - base);
-      sum += sl[q] * x;
-      acc += so[q][t] * x;
+      for (int i = 0; i < kAhead; ++i) {
+        const float big = fmaxf(m, pm[i]), base = big == -INFINITY ? 0.0f : big;
+        const float ca = exp2_fast(m - base), cb = exp2_fast(pm[i] - base);
+        l = l * ca + pl[i] * cb;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) o[k] = o[k] * ca + po[i][k] * cb;
+        m = big;
+      }
     }
-    const float y = acc * (sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum);
-    op[t] = BF16 ? pq_f32_to_bf16(y) : pq_f32_to_f16(y);
-    if (t == 0) *lse = (big + log2_fast(sum)) * kLn2;
+  };
+  const auto write = [&](int h, float m, float l, const float (&o)[kV]) {
+    const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+#pragma unroll
+    for (int k = 0; k < kV; ++k)
+      out_row(h)[lane * kV + k] = BF16 ? pq_f32_to_bf16(o[k] * inv) : pq_f32_to_f16(o[k] * inv);
+    if (lane == 0) *lse_of(h) = (m + log2_fast(l)) * kLn2;
+  };
+
+  // heads of a unit's rows share their parts but not their first one: whether they are many is the same for all of them
+  if ((static_cast<int64_t>(npages) * n) / total <= 16) {
+    const int h = blockIdx.y * kWaves + wave;
+    if (h >= hq) return;
+    const Parts q = parts_of(h);
+    if (q.w0 == q.w1) return;   // written by the workgroup that had all of it
+    float m, l, o[kV];
+    gather(q, 0, 1, m, l, o);
+    write(h, m, l, o);
+    return;
+  }
+  for (int i = 0; i < kWaves; ++i) {
+    const int h = blockIdx.y * kWaves + i;
+    if (h >= hq) return;
+    const Parts q = parts_of(h);
+    float m, l, o[kV];
+    gather(q, wave, kWaves, m, l, o);
+    if (lane == 0) {
+      sm[wave] = m;
+      sl[wave] = l;
+    }
+#pragma unroll
+    for (int k = 0; k < kV; ++k) so[wave][lane * kV + k] = o[k];
+    __syncthreads();
+    if (wave == 0) {
+      float big = sm[0];
+#pragma unroll
+      for (int x = 1; x < kWaves; ++x) big = fmaxf(big, sm[x]);
+      const float base = big == -INFINITY ? 0.0f : big;
+      l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kV; ++k) o[k] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kWaves; ++x) {
+        const float f = exp2_fast(sm[x] - base);
+        l += sl[x] * f;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) o[k] += so[x][lane * kV + k] * f;
+      }
+      write(h, big, l, o);
+    }
+    __syncthreads();
   }
 }
 
@@ -536,12 +644,12 @@ extern "C" int pq_attn_cache_i8(const void* q, int dtype, int64_t q_stride_token
   a.pages = static_cast<int>(pages); a.workers = kWorkers;
   a.scale_log2 = scale * kLog2e;
   const int rt = batch > 0 ? row_tiles(batch, tokens, group) : 1;
-  const dim3 join(static_cast<unsigned>(tokens), static_cast<unsigned>(kv_heads * group));
+  const dim3 join(static_cast<unsigned>(tokens), static_cast<unsigned>((kv_heads * group + kWaves - 1) / kWaves));
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define PQ_CACHE(D_, RT_, BF_)                                                    \
   do {                                                                            \
     if (a.batch > 0 && a.width > 0)                                               \
-      attn_cache_kernel<D_, RT_, BF_><<<kWorkers, kThreads, 0, s>>>(a);           \
+      attn_cache_kernel<D_, (RT_ == 1 ? 1 : kRT), (RT_ == 1 ? 1 : RT_ / kRT), BF_><<<a.workers, kThreads, 0, s>>>(a);           \
     attn_cache_join_kernel<D_, RT_, BF_><<<join, kThreads, 0, s>>>(a);            \
   } while (0)
 #define PQ_CACHE_RT(D_, BF_)                 \
