@@ -38,10 +38,6 @@ using namespace pqa;
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kWorkers = 512;
-#ifndef KRT
-#define KRT 1
-#endif
-constexpr int kRT = KRT;
 
 struct CacheArgs {
   const void* q;                      // [tokens, heads * group, d]
@@ -65,26 +61,39 @@ __device__ __forceinline__ int seq_len(const CacheArgs& a, int b) {
   return min(max(a.lens[b], 0), a.width * kPage);
 }
 
-// A unit: kRows rows of a sequence and head.  Units of a sequence are ordered by tile, then by head.
+// A unit: ROWS rows of a sequence and head.  Units of a sequence are ordered by tile, then by head.  A unit counts as its
+// pages and kLead more, which stand for what it costs to begin and end one.
+constexpr int kLead = 4;
+
 template <int ROWS>
 struct Plan {
-  // pages that sequence b's units read in all
+  static __device__ __forceinline__ int64_t size(int npages) { return npages > 0 ? npages + kLead : 0; }
+  // what sequence b's units count in all
   static __device__ __forceinline__ int64_t cost(const CacheArgs& a, int b) {
     const int64_t rows = static_cast<int64_t>(span_of(a.cu, b, a.tokens).count) * a.group;
-    return (rows + ROWS - 1) / ROWS * a.heads * ((seq_len(a, b) + kPage - 1) / kPage);
+    return (rows + ROWS - 1) / ROWS * a.heads * size((seq_len(a, b) + kPage - 1) / kPage);
   }
-  // Workgroups that take part: each has work for its waves.
-  static __device__ __forceinline__ int64_t workers(const CacheArgs& a, int64_t total) {
-    const int64_t w = (total + kWaves - 1) / kWaves;
-    return w < a.workers ? w : a.workers;
+};
+
+// Quotient of non-negative numbers, in 32 bits where they allow it (the 64-bit division is a hundred instructions).
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return x / y;
+}
+
+// `total` numbers in shares for n workgroups, of each + 1 numbers for the first `more` and `each` for the others.
+struct Shares {
+  int64_t n, each, more;
+  __device__ __forceinline__ Shares(int64_t total, int workers) {
+    n = min(static_cast<int64_t>(workers), (total + kWaves - 1) / kWaves);   // each has work for its waves
+    each = n > 0 ? quotient(total, n) : 0;
+    more = total - each * n;
   }
-  static __device__ __forceinline__ int64_t begin(int64_t w, int64_t total, int64_t n) { return w * total / n; }
-  // The workgroup whose share holds page x.
-  static __device__ __forceinline__ int64_t owner(int64_t x, int64_t total, int64_t n) {
-    int64_t w = x * n / total;
-    while (begin(w + 1, total, n) <= x) ++w;
-    while (begin(w, total, n) > x) --w;
-    return w;
+  __device__ __forceinline__ int64_t begin(int64_t w) const { return w * each + min(w, more); }
+  // the workgroup whose share holds number x
+  __device__ __forceinline__ int64_t owner(int64_t x) const {
+    const int64_t wide = more * (each + 1);
+    return x < wide ? quotient(x, each + 1) : more + quotient(x - wide, each);
   }
 };
 
@@ -131,249 +140,376 @@ __device__ __forceinline__ void load_q(const CacheArgs& a, int first, int rows, 
   mult = down * a.scale_log2;
 }
 
-// The K codes of a page: tile t's row r is token at(t, r), 2 x 16 bytes of it (d = 64: 1) for each lane.
+// The K codes of tile t of a page, 2 x 16 bytes (d = 64: 1) for each lane.  INTERLEAVED: row r of the tile is token
+// 16 (r / 4) + 4 t + r % 4, so that a lane of the product gets neighbouring tokens from the four tiles.
 template <int D, bool INTERLEAVED>
-__device__ __forceinline__ void load_k(const int8_t* page, u4 (&kr)[4][D / 64]) {
+__device__ __forceinline__ void load_k(const int8_t* page, int t, u4 (&kr)[D / 64]) {
   const int lane = lane_id(), g = lane >> 4, r = lane & 15;
+  const int token = INTERLEAVED ? 16 * (r >> 2) + 4 * t + (r & 3) : 16 * t + r;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int token = INTERLEAVED ? 16 * (r >> 2) + 4 * t + (r & 3) : 16 * t + r;
+  for (int i = 0; i < D / 64; ++i) kr[i] = *reinterpret_cast<const u4*>(page + token * D + i * 64 + g * 16);
+}
+
+// 16 rows of a unit: their queries, running maximum and sum, and results.  Lane: row lane & 15.
+template <int D, bool BF16>
+struct Rows16 {
+  static constexpr int kDt = D / 16;
+  h8 qf[D / 32];
+  float mult, m, l;
+  int limit, sure;      // keys that the lane's row sees, and that every one of the rows sees
+  f4 o[kDt];
+
+  __device__ __forceinline__ void begin(const CacheArgs& a, const Span& sp, int len, int rows, int head, int row0) {
+    load_q<D, BF16>(a, sp.first, rows, head, row0, qf, mult);
+    limit = min((row0 + (lane_id() & 15)) / a.group + len - sp.count + 1, len);
+    sure = row0 / a.group + len - sp.count + 1;
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) kr[t][i] = *reinterpret_cast<const u4*>(page + token * D + i * 64 + g * 16);
+    for (int k = 0; k < kDt; ++k) o[k] = f4{0, 0, 0, 0};
+  }
+
+  // Scores of a page, as tokens 16 g + 4 q + e of lane group g, to weights.  see: tokens of the page that the lane's row
+  // sees, where masked.
+  __device__ __forceinline__ void weigh(f4 (&s)[4], float ks, bool masked, int see, h8 (&pf)[2]) {
+    // never 0: what is masked stays -inf, and scores of rows and pages of zeros stay as good as 0
+    const float c = fmaxf(ks * mult, 1e-37f);
+    if (masked) {
+      see -= 16 * (lane_id() >> 4);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[q][e] = 4 * q + e >= see ? -INFINITY : s[q][e];
+    }
+    float big = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) big = fmaxf(big, s[q][e]);
+    // a row's maximum moves by more than 8 (in base 2) at a time, each row by itself
+    big = max_xor32(max_xor16(big)) * c;
+    const bool moves = big > m + 8.0f;
+    if (__any(moves)) {
+      const float now = moves ? big : m;
+      const float alpha = moves ? exp2_fast(m - now) : 1.0f;
+      m = now;
+      l *= alpha;
+#pragma unroll
+      for (int k = 0; k < kDt; ++k) o[k] *= alpha;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      u4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = exp2_fast(__builtin_fmaf(s[2 * q + (e >> 1)][2 * (e & 1)], c, -base));
+        const float y = exp2_fast(__builtin_fmaf(s[2 * q + (e >> 1)][2 * (e & 1) + 1], c, -base));
+        sum += x + y;
+        w[e] = pqd::pk_f16(x, y);
+      }
+      pf[q] = __builtin_bit_cast(h8, w);
+    }
+    l += sum;
+  }
+
+  // Results of channels 16 k + 4 g + 0..3 from the page's values (two operands) and weights.
+  __device__ __forceinline__ void add(int k, const h8& v0, const h8& v1, const h8 (&pf)[2], float vs) {
+    f4 x = {0, 0, 0, 0};
+    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[0], x, 0, 0, 0);
+    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[1], x, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[k][e] = __builtin_fmaf(x[e], vs, o[k][e]);
+  }
+};
+
+// A share's segment: pages [p0, p1) of a unit.
+struct Segment {
+  Span sp;
+  int b, len, npages, rows, head, row0, p0, p1;
+  bool first;           // of its share
+};
+
+// Calls f for the segments of workgroup blockIdx.x's share, in order.
+template <int ROWS, class F>
+__device__ __forceinline__ void for_segments(const CacheArgs& a, F f) {
+  using P = Plan<ROWS>;
+  const auto cost = [&](int b) { return P::cost(a, b); };
+  const int64_t total = sum_seqs(a.batch, cost);
+  const Shares shares(total, a.workers);
+  const int64_t w = blockIdx.x;
+  if (w >= shares.n) return;
+  const int64_t from = shares.begin(w), to = shares.begin(w + 1);
+  for (int64_t at = from; at < to;) {
+    const Found fd = find_seq(a.batch, at, cost);
+    if (fd.b < 0) break;
+    Segment s;
+    s.b = fd.b;
+    s.sp = span_of(a.cu, fd.b, a.tokens);
+    s.len = seq_len(a, fd.b);
+    s.npages = (s.len + kPage - 1) / kPage;
+    s.rows = s.sp.count * a.group;
+    const int64_t size = P::size(s.npages);
+    const int unit = static_cast<int>(quotient(fd.local, size)), x0 = static_cast<int>(fd.local - unit * size);
+    const int x1 = static_cast<int>(min(size, x0 + (to - at)));
+    s.head = unit % a.heads;
+    s.row0 = unit / a.heads * ROWS;
+    s.p0 = max(0, x0 - kLead);
+    s.p1 = x1 - kLead;
+    s.first = at == from;
+    at += x1 - x0;
+    if (s.p0 < s.p1) f(s);   // else none of the unit's pages
   }
 }
 
-// RT row tiles of 16 for each wave, RW waves with rows of their own on the same pages.
-template <int D, int RT, int RW, bool BF16>
-__global__ __launch_bounds__(kThreads, RT == 4 ? 1 : 2) void attn_cache_kernel(CacheArgs a) {
-  constexpr int kRows = 16 * RT * RW, kDt = D / 16, kStreams = kWaves / RW;
-  constexpr int kPitch = D + 4;
+// page * heads + head; a number that is no page: page 0, with no token to see
+__device__ __forceinline__ int64_t page_head(const CacheArgs& a, int id, int head) {
+  return static_cast<int64_t>(id < 0 || id >= a.pages ? 0 : id) * a.heads + head;
+}
+
+// Where a row of a segment goes: to the outputs, if the segment is all of its unit, else to the partial results.
+template <int ROWS, int D, bool BF16>
+struct Dest {
+  uint16_t* out;
+  float *lse, *part;
+  __device__ __forceinline__ Dest(const CacheArgs& a, const Segment& s, int r) {
+    const int row = s.row0 + r;
+    part = nullptr;
+    if (s.p0 == 0 && s.p1 == s.npages) {
+      const int token = s.sp.first + row / a.group, h = s.head * a.group + row % a.group;
+      out = static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(token) * a.heads * a.group + h) * D;
+      lse = a.lse + static_cast<int64_t>(h) * a.tokens + token;
+    } else {
+      float* base = a.part + (2 * static_cast<int64_t>(blockIdx.x) + (s.first ? 0 : 1)) * part_floats<ROWS, D>();
+      part = base + r * D;
+      lse = base + ROWS * D + r;
+    }
+  }
+  // Channels c .. c + 3 of a row whose weights sum to `sum`.
+  __device__ __forceinline__ void put(int c, const f4& x, float sum) const {
+    if (part) {
+      *reinterpret_cast<f4*>(part + c) = x;
+      return;
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
+    uint16_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = BF16 ? pq_f32_to_bf16(x[e] * inv) : pq_f32_to_f16(x[e] * inv);
+    *reinterpret_cast<uint2*>(out + c) = make_uint2(y[0] | static_cast<uint32_t>(y[1]) << 16, y[2] | static_cast<uint32_t>(y[3]) << 16);
+  }
+  __device__ __forceinline__ void put_stats(float m, float sum) const {
+    if (part) {
+      lse[0] = m;
+      lse[ROWS] = sum;
+    } else {
+      *lse = (m + log2_fast(sum)) * kLn2;
+    }
+  }
+};
+
+// Units of 16 rows: every wave carries them all and takes every fourth page of a segment.
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void attn_cache_kernel(CacheArgs a) {
+  constexpr int kDt = D / 16, kPitch = D + 4;
   __shared__ __align__(16) float so[kWaves][16][kPitch];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
-  using P = Plan<kRows>;
   const int t = threadIdx.x, lane = t & 63, g = lane >> 4, col = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), stream = wave / RW, part_of = wave % RW;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
 
-  const auto cost = [&](int b) { return P::cost(a, b); };
-  const int64_t total = sum_seqs(a.batch, cost);
-  const int64_t n = P::workers(a, total), w = blockIdx.x;
-  if (w >= n) return;
-  const int64_t from = P::begin(w, total, n), to = P::begin(w + 1, total, n);
-
-  for (int64_t at = from; at < to;) {
-    const Found f = find_seq(a.batch, at, cost);
-    if (f.b < 0) break;
-    const Span sp = span_of(a.cu, f.b, a.tokens);
-    const int len = seq_len(a, f.b), npages = (len + kPage - 1) / kPage;
-    const int rows = sp.count * a.group;
-    const int unit = static_cast<int>(f.local / npages), p0 = static_cast<int>(f.local % npages);
-    const int head = unit % a.heads, row0 = unit / a.heads * kRows;
-    const int p1 = static_cast<int>(min(static_cast<int64_t>(npages), p0 + (to - at)));
-
-    h8 qf[RT][D / 32];
-    float mult[RT];
-    int limit[RT];     // keys that the lane's row sees
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const int first = row0 + 16 * (RT * part_of + i);
-      load_q<D, BF16>(a, sp.first, rows, head, first, qf[i], mult[i]);
-      limit[i] = min((first + col) / a.group + len - sp.count + 1, len);
-    }
-    const int sure = (row0 + 16 * RT * part_of) / a.group + len - sp.count + 1;   // keys that every row of the wave sees
-
-    float m[RT], l[RT];
-    f4 o[RT][kDt];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      m[i] = -INFINITY;
-      l[i] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < kDt; ++k) o[i][k] = f4{0, 0, 0, 0};
-    }
+  for_segments<16>(a, [&](const Segment& sg) {
+    Rows16<D, BF16> rw;
+    rw.begin(a, sg.sp, sg.len, sg.rows, sg.head, sg.row0);
 
     // The next page's codes are asked for as soon as the registers of this one's are free: K behind the first product,
     // V behind the second; its number one page ahead of that.
-    const int* table = a.table + static_cast<int64_t>(f.b) * a.width;
+    const int* table = a.table + static_cast<int64_t>(sg.b) * a.width;
     u4 kr[4][D / 64], vr[kDt];
-    float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
     const auto load_v = [&](int64_t ph) {
       const int8_t* vp = a.vc + ph * (kPage * D);
 #pragma unroll
       for (int k = 0; k < kDt; ++k) vr[k] = *reinterpret_cast<const u4*>(vp + (16 * k + col) * kPage + g * 16);
     };
-    const auto number = [&](int p) { return scalar_load(table + p); };
-    // page and head of place p; a number that is no page: page 0, with no token to see
-    const auto page_head = [&](int id) { return static_cast<int64_t>(id < 0 || id >= a.pages ? 0 : id) * a.heads + head; };
-
-    // seen: tokens of the cache that rows may see; masked: some row does not see some token of the page
-    const auto step = [&](bool masked, int seen, int p, int64_t ph_next) {
-      ks_next = scalar_load(a.ks + ph_next);
-      vs_next = scalar_load(a.vs + ph_next);
-      f4 s[RT][4];
+    int p = sg.p0 + wave;
+    if (p < sg.p1) {
+      int id = scalar_load(table + p), id_next = p + kWaves < sg.p1 ? scalar_load(table + p + kWaves) : 0;
+      int64_t ph = page_head(a, id, sg.head);
+      float ks = scalar_load(a.ks + ph), vs = scalar_load(a.vs + ph);
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) s[i][q] = f4{0, 0, 0, 0};
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const h8 kf = codes_f16(kr[q][k >> 1][2 * (k & 1)], kr[q][k >> 1][2 * (k & 1) + 1]);
-#pragma unroll
-          for (int i = 0; i < RT; ++i) s[i][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[i][k], s[i][q], 0, 0, 0);
-        }
-      load_k<D, true>(a.kc + ph_next * (kPage * D), kr);
-      __builtin_amdgcn_sched_barrier(0);
-
-      // the lane's tokens: 16 g + 4 q + e
-      h8 pf[RT][2];
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        // never 0: what is masked stays -inf, and scores of rows and pages of zeros stay as good as 0
-        const float c = fmaxf(ks * mult[i], 1e-37f);
-        float big = -INFINITY;
-        if (masked) {
-          const int see = min(limit[i], seen) - p * kPage - 16 * g;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][q][e] = 4 * q + e >= see ? -INFINITY : s[i][q][e];
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) big = fmaxf(big, s[i][q][e]);
-        // a row's maximum moves by more than 8 (in base 2) at a time, each row by itself
-        big = max_xor32(max_xor16(big)) * c;
-        const bool moves = big > m[i] + 8.0f;
-        if (__any(moves)) {
-          const float now = moves ? big : m[i];
-          const float alpha = moves ? exp2_fast(m[i] - now) : 1.0f;
-          m[i] = now;
-          l[i] *= alpha;
-#pragma unroll
-          for (int k = 0; k < kDt; ++k) o[i][k] *= alpha;
-        }
-        const float base = m[i] == -INFINITY ? 0.0f : m[i];
-        float sum = 0.0f;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          u4 w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = exp2_fast(__builtin_fmaf(s[i][2 * q + (e >> 1)][2 * (e & 1)], c, -base));
-            const float y = exp2_fast(__builtin_fmaf(s[i][2 * q + (e >> 1)][2 * (e & 1) + 1], c, -base));
-            sum += x + y;
-            w[e] = pqd::pk_f16(x, y);
-          }
-          pf[i][q] = __builtin_bit_cast(h8, w);
-        }
-        l[i] += sum;
-      }
-#pragma unroll
-      for (int k = 0; k < kDt; ++k) {
-        const h8 v0 = codes_f16(vr[k][0], vr[k][1]), v1 = codes_f16(vr[k][2], vr[k][3]);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          f4 x = {0, 0, 0, 0};
-          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[i][0], x, 0, 0, 0);
-          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[i][1], x, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][k][e] = __builtin_fmaf(x[e], vs, o[i][k][e]);
-        }
-      }
-      load_v(ph_next);
-      __builtin_amdgcn_sched_barrier(0);
-    };
-
-    int p = p0 + stream;
-    if (p < p1) {
-      int id = number(p), id_next = p + kStreams < p1 ? number(p + kStreams) : 0;
-      const int64_t ph = page_head(id);
-      ks = scalar_load(a.ks + ph);
-      vs = scalar_load(a.vs + ph);
-      load_k<D, true>(a.kc + ph * (kPage * D), kr);
+      for (int q = 0; q < 4; ++q) load_k<D, true>(a.kc + ph * (kPage * D), q, kr[q]);
       __builtin_amdgcn_sched_barrier(0);   // K before V, as in the loop: the wait for K then leaves V in flight
       load_v(ph);
       __builtin_amdgcn_sched_barrier(0);
-      for (; p < p1; p += kStreams) {
+      for (; p < sg.p1; p += kWaves) {
         // behind the last page the loads, which the waits count on, go to that page again
         const bool there = id >= 0 && id < a.pages;
-        id = p + kStreams < p1 ? id_next : id;
-        const int64_t ph_next = page_head(id);
-        if (p + 2 * kStreams < p1) id_next = number(p + 2 * kStreams);
-        step(!there || (p + 1) * kPage > sure, there ? len : 0, p, ph_next);
+        id = p + kWaves < sg.p1 ? id_next : id;
+        ph = page_head(a, id, sg.head);
+        if (p + 2 * kWaves < sg.p1) id_next = scalar_load(table + p + 2 * kWaves);
+        const float ks_next = scalar_load(a.ks + ph), vs_next = scalar_load(a.vs + ph);
+        f4 s[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            s[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                codes_f16(kr[q][k >> 1][2 * (k & 1)], kr[q][k >> 1][2 * (k & 1) + 1]), rw.qf[k], s[q], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) load_k<D, true>(a.kc + ph * (kPage * D), q, kr[q]);
+        __builtin_amdgcn_sched_barrier(0);
+        h8 pf[2];
+        rw.weigh(s, ks, !there || (p + 1) * kPage > rw.sure, (there ? rw.limit : 0) - p * kPage, pf);
+#pragma unroll
+        for (int k = 0; k < kDt; ++k) rw.add(k, codes_f16(vr[k][0], vr[k][1]), codes_f16(vr[k][2], vr[k][3]), pf, vs);
+        load_v(ph);
+        __builtin_amdgcn_sched_barrier(0);
         ks = ks_next;
         vs = vs_next;
       }
     }
 
-    // the results of the segment, from the waves that went through its pages
-    const bool whole = p0 == 0 && p1 == npages;
-    float* part = a.part + (2 * w + (at == from ? 0 : 1)) * part_floats<kRows, D>();
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const float lt = sum_xor32(sum_xor16(l[i]));
-      if (g == 0) {
-        sm[wave][col] = m[i];
-        sl[wave][col] = lt;
-      }
-#pragma unroll
-      for (int k = 0; k < kDt; ++k) *reinterpret_cast<f4*>(&so[wave][col][16 * k + 4 * g]) = o[i][k];
-      __syncthreads();
-#pragma unroll
-      for (int x = 0; x < RW; ++x) {
-        const int r = t >> 4, local = 16 * (RT * x + i) + r, row = row0 + local;
-        if (row >= rows) continue;
-        float big = sm[x][r];
-#pragma unroll
-        for (int q = 1; q < kStreams; ++q) big = fmaxf(big, sm[RW * q + x][r]);
-        const float base = big == -INFINITY ? 0.0f : big;
-        float sum = 0.0f;
-        f4 acc[D / 64];
-#pragma unroll
-        for (int k = 0; k < D / 64; ++k) acc[k] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int q = 0; q < kStreams; ++q) {
-          const float y = exp2_fast(sm[RW * q + x][r] - base);
-          sum += sl[RW * q + x][r] * y;
-#pragma unroll
-          for (int k = 0; k < D / 64; ++k) acc[k] += *reinterpret_cast<const f4*>(&so[RW * q + x][r][64 * k + 4 * (t & 15)]) * y;
-        }
-        if (whole) {
-          const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
-          const int token = sp.first + row / a.group, h = head * a.group + row % a.group;
-          uint16_t* op = static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(token) * a.heads * a.group + h) * D;
-#pragma unroll
-          for (int k = 0; k < D / 64; ++k) {
-            uint16_t y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = BF16 ? pq_f32_to_bf16(acc[k][e] * inv) : pq_f32_to_f16(acc[k][e] * inv);
-            *reinterpret_cast<uint2*>(op + 64 * k + 4 * (t & 15)) =
-                make_uint2(y[0] | static_cast<uint32_t>(y[1]) << 16, y[2] | static_cast<uint32_t>(y[3]) << 16);
-          }
-          if ((t & 15) == 0) a.lse[static_cast<int64_t>(h) * a.tokens + token] = (big + log2_fast(sum)) * kLn2;
-        } else {
-#pragma unroll
-          for (int k = 0; k < D / 64; ++k) *reinterpret_cast<f4*>(part + local * D + 64 * k + 4 * (t & 15)) = acc[k];
-          if ((t & 15) == 0) {
-            part[kRows * D + local] = big;
-            part[kRows * D + kRows + local] = sum;
-          }
-        }
-      }
-      __syncthreads();
+    // the results of the segment from the four waves
+    const float lt = sum_xor32(sum_xor16(rw.l));
+    if (g == 0) {
+      sm[wave][col] = rw.m;
+      sl[wave][col] = lt;
     }
-    at += p1 - p0;
-  }
+#pragma unroll
+    for (int k = 0; k < kDt; ++k) *reinterpret_cast<f4*>(&so[wave][col][16 * k + 4 * g]) = rw.o[k];
+    __syncthreads();
+    const int r = t >> 4, row = sg.row0 + r, c4 = 4 * (t & 15);
+    if (row < sg.rows) {
+      float big = sm[0][r];
+#pragma unroll
+      for (int q = 1; q < kWaves; ++q) big = fmaxf(big, sm[q][r]);
+      const float base = big == -INFINITY ? 0.0f : big;
+      float sum = 0.0f;
+      f4 acc[D / 64];
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) acc[k] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int q = 0; q < kWaves; ++q) {
+        const float y = exp2_fast(sm[q][r] - base);
+        sum += sl[q][r] * y;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) acc[k] += *reinterpret_cast<const f4*>(&so[q][r][64 * k + c4]) * y;
+      }
+      Dest<16, D, BF16> out(a, sg, r);
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) out.put(64 * k + c4, acc[k], sum);
+      if ((t & 15) == 0) out.put_stats(big, sum);
+    }
+    __syncthreads();
+  });
+}
+
+// Units of 64 rows, 16 a wave: a page's codes become operands once, a quarter by each wave, and pass to the others
+// through LDS in the order in which lanes take them.  A wave asks for its quarter of a page three pages ahead.
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void attn_cache_rows_kernel(CacheArgs a) {
+  constexpr int kDt = D / 16, kKs = D / 32, kEach = D / 64;
+  __shared__ h8 kf[2][4][kKs][64], vf[2][kDt][2][64];
+  const int t = threadIdx.x, lane = t & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+
+  for_segments<64>(a, [&](const Segment& sg) {
+    Rows16<D, BF16> rw;
+    const int r0 = sg.row0 + 16 * wave;
+    rw.begin(a, sg.sp, sg.len, sg.rows, sg.head, r0);
+    const int* table = a.table + static_cast<int64_t>(sg.b) * a.width;
+    // behind the last page the loads, which the waits count on, go to that page again
+    const auto number = [&](int p) { return scalar_load(table + min(p, sg.p1 - 1)); };
+    struct Raw { u4 k[kEach], v[kEach]; };
+    const auto load = [&](int id, Raw& x) {
+      const int64_t ph = page_head(a, id, sg.head);
+      load_k<D, true>(a.kc + ph * (kPage * D), wave, x.k);
+      const int8_t* vp = a.vc + ph * (kPage * D);
+#pragma unroll
+      for (int k = 0; k < kEach; ++k)
+        x.v[k] = *reinterpret_cast<const u4*>(vp + (16 * (kEach * wave + k) + col) * kPage + g * 16);
+    };
+    const auto spread = [&](const Raw& x, int to) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          kf[to][wave][2 * i + h][lane] = codes_f16(x.k[i][2 * h], x.k[i][2 * h + 1]);
+          vf[to][kEach * wave + i][h][lane] = codes_f16(x.v[i][2 * h], x.v[i][2 * h + 1]);
+        }
+    };
+
+    int p = sg.p0;
+    int id[4];           // pages p .. p + 3
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = number(p + i);
+    Raw x0, x1;
+    load(id[0], x0);
+    __builtin_amdgcn_sched_barrier(0);
+    load(id[1], x1);
+    __builtin_amdgcn_sched_barrier(0);
+    int64_t ph = page_head(a, id[0], sg.head);
+    float ks = scalar_load(a.ks + ph), vs = scalar_load(a.vs + ph);
+    spread(x0, 0);
+    load(id[2], x0);
+    __builtin_amdgcn_sched_barrier(0);
+    pqd::lds_barrier();
+
+    // page p from stage `from`; x: page p + 1, then p + 3
+    const auto step = [&](Raw& x, int from) {
+      spread(x, from ^ 1);
+      load(id[3], x);
+      __builtin_amdgcn_sched_barrier(0);
+      ph = page_head(a, id[1], sg.head);
+      const float ks_next = scalar_load(a.ks + ph), vs_next = scalar_load(a.vs + ph);
+      const bool there = id[0] >= 0 && id[0] < a.pages;
+      id[0] = id[1];
+      id[1] = id[2];
+      id[2] = id[3];
+      id[3] = number(p + 4);
+      if (r0 < sg.rows) {
+        f4 s[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < kKs; ++k)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            s[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[from][q][k][lane], rw.qf[k], s[q], 0, 0, 0);
+        h8 pf[2];
+        rw.weigh(s, ks, !there || (p + 1) * kPage > rw.sure, (there ? rw.limit : 0) - p * kPage, pf);
+#pragma unroll
+        for (int k = 0; k < kDt; ++k) rw.add(k, vf[from][k][0][lane], vf[from][k][1][lane], pf, vs);
+      }
+      ks = ks_next;
+      vs = vs_next;
+      pqd::lds_barrier();
+    };
+    while (p < sg.p1) {
+      step(x1, 0);
+      ++p;
+      if (p >= sg.p1) break;
+      step(x0, 1);
+      ++p;
+    }
+
+    const float lt = sum_xor32(sum_xor16(rw.l));
+    if (r0 + col < sg.rows) {
+      Dest<64, D, BF16> out(a, sg, 16 * wave + col);
+#pragma unroll
+      for (int k = 0; k < kDt; ++k) out.put(16 * k + 4 * g, rw.o[k], lt);
+      if (g == 0) out.put_stats(rw.m, lt);
+    }
+  });
 }
 
 // Joins the partial results of the rows whose unit spans workgroups.  A workgroup takes four (query head, token) rows of a
 // token: a wave each, or, where the parts are many, its waves together on one row after the other.  Rows outside of the
 // sequences and rows of empty ones get zeros and lse = -inf.
-template <int D, int RT, bool BF16>
+template <int D, int kRows, bool BF16>
 __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) {
-  constexpr int kRows = 16 * RT, kV = D / 64;
+  constexpr int kV = D / 64;
   __shared__ float so[kWaves][D], sl[kWaves], sm[kWaves];
   using P = Plan<kRows>;
   const int token = blockIdx.x, t = threadIdx.x, lane = t & 63;
@@ -412,16 +548,16 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
   }
   const Span sp = span_of(a.cu, b, a.tokens);
   const int npages = (len + kPage - 1) / kPage;
-  const int64_t n = P::workers(a, total);
+  const Shares shares(total, a.workers);
 
   // parts w0 + first, w0 + first + step, ... of a row into m, l, o
   struct Parts { int64_t begin, w0, w1; int r; };
   const auto parts_of = [&](int h) {
     const int head = h / a.group, row = (token - sp.first) * a.group + h - head * a.group;
     Parts q;
-    q.begin = before + (static_cast<int64_t>(row / kRows) * a.heads + head) * npages;
-    q.w0 = P::owner(q.begin, total, n);
-    q.w1 = P::owner(q.begin + npages - 1, total, n);
+    q.begin = before + (static_cast<int64_t>(row / kRows) * a.heads + head) * P::size(npages);
+    q.w0 = shares.owner(q.begin + kLead);
+    q.w1 = shares.owner(q.begin + kLead + npages - 1);
     q.r = row % kRows;
     return q;
   };
@@ -441,7 +577,7 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
         for (int k = 0; k < kV; ++k) po[i][k] = 0.0f;
         const int64_t x = w + i * step;
         if (x <= q.w1) {
-          const bool own = x > q.w0 || P::begin(x, total, n) == q.begin;
+          const bool own = shares.begin(x) >= q.begin;   // the unit is the first of its share
           const float* p = a.part + (2 * x + (own ? 0 : 1)) * part_floats<kRows, D>();
           pm[i] = p[kRows * D + q.r];
           pl[i] = p[kRows * D + kRows + q.r];
@@ -469,7 +605,7 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
   };
 
   // heads of a unit's rows share their parts but not their first one: whether they are many is the same for all of them
-  if ((static_cast<int64_t>(npages) * n) / total <= 16) {
+  if (npages <= 16 * shares.each) {
     const int h = blockIdx.y * kWaves + wave;
     if (h >= hq) return;
     const Parts q = parts_of(h);
@@ -537,7 +673,8 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheArgs a) {
     if (page < 0 || page >= a.pages) continue;
     const int64_t ph = static_cast<int64_t>(page) * a.heads + head;
     u4 kr[4][D / 64];
-    load_k<D, false>(a.kc + ph * (kPage * D), kr);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) load_k<D, false>(a.kc + ph * (kPage * D), q, kr[q]);
     const float ks = a.ks[ph];
     h8 kf[4][D / 32];
 #pragma unroll
@@ -583,11 +720,8 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheArgs a) {
   }
 }
 
-// Row tiles of 16 that a unit carries: enough for the call's average rows, at most 4.
-int row_tiles(int64_t batch, int64_t tokens, int64_t group) {
-  const int64_t rows = (tokens * group + batch - 1) / batch;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-}
+// Rows of a unit: 16 where the call's sequences have no more on the average, else 64.
+int unit_rows(int64_t batch, int64_t tokens, int64_t group) { return tokens * group <= 16 * batch ? 16 : 64; }
 
 int check(const char* who, const void* q, int dtype, int64_t q_st, int64_t q_sh, const void* k_cache, const void* k_scale,
           const void* table, const void* cu, const void* lens, int64_t batch, int64_t width, int64_t tokens,
@@ -615,7 +749,7 @@ int check(const char* who, const void* q, int dtype, int64_t q_st, int64_t q_sh,
 
 extern "C" size_t pq_attn_cache_i8_workspace_size(int64_t batch, int64_t tokens, int64_t group, int64_t head_dim) {
   if (batch <= 0 || tokens <= 0 || group <= 0 || head_dim <= 0) return 0;
-  return static_cast<size_t>(2 * kWorkers) * (16 * row_tiles(batch, tokens, group)) * (head_dim + 2) * sizeof(float);
+  return static_cast<size_t>(2 * kWorkers) * unit_rows(batch, tokens, group) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int pq_attn_cache_i8(const void* q, int dtype, int64_t q_stride_token, int64_t q_stride_head,
@@ -643,26 +777,22 @@ extern "C" int pq_attn_cache_i8(const void* q, int dtype, int64_t q_stride_token
   a.tokens = static_cast<int>(tokens); a.heads = static_cast<int>(kv_heads); a.group = static_cast<int>(group);
   a.pages = static_cast<int>(pages); a.workers = kWorkers;
   a.scale_log2 = scale * kLog2e;
-  const int rt = batch > 0 ? row_tiles(batch, tokens, group) : 1;
+  const bool few = batch == 0 || unit_rows(batch, tokens, group) == 16;
   const dim3 join(static_cast<unsigned>(tokens), static_cast<unsigned>((kv_heads * group + kWaves - 1) / kWaves));
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define PQ_CACHE(D_, RT_, BF_)                                                    \
-  do {                                                                            \
-    if (a.batch > 0 && a.width > 0)                                               \
-      attn_cache_kernel<D_, (RT_ == 1 ? 1 : kRT), (RT_ == 1 ? 1 : RT_ / kRT), BF_><<<a.workers, kThreads, 0, s>>>(a);           \
-    attn_cache_join_kernel<D_, RT_, BF_><<<join, kThreads, 0, s>>>(a);            \
+#define PQ_CACHE(D_, BF_)                                                          \
+  do {                                                                             \
+    if (a.batch > 0 && a.width > 0) {                                              \
+      if (few) attn_cache_kernel<D_, BF_><<<kWorkers, kThreads, 0, s>>>(a);        \
+      else attn_cache_rows_kernel<D_, BF_><<<kWorkers, kThreads, 0, s>>>(a);       \
+    }                                                                              \
+    if (few) attn_cache_join_kernel<D_, 16, BF_><<<join, kThreads, 0, s>>>(a);     \
+    else attn_cache_join_kernel<D_, 64, BF_><<<join, kThreads, 0, s>>>(a);         \
   } while (0)
-#define PQ_CACHE_RT(D_, BF_)                 \
-  do {                                       \
-    if (rt == 1) PQ_CACHE(D_, 1, BF_);       \
-    else if (rt == 2) PQ_CACHE(D_, 2, BF_);  \
-    else PQ_CACHE(D_, 4, BF_);               \
-  } while (0)
-  if (head_dim == 64 && dtype == PQ_BF16) PQ_CACHE_RT(64, true);
-  else if (head_dim == 64) PQ_CACHE_RT(64, false);
-  else if (dtype == PQ_BF16) PQ_CACHE_RT(128, true);
-  else PQ_CACHE_RT(128, false);
-#undef PQ_CACHE_RT
+  if (head_dim == 64 && dtype == PQ_BF16) PQ_CACHE(64, true);
+  else if (head_dim == 64) PQ_CACHE(64, false);
+  else if (dtype == PQ_BF16) PQ_CACHE(128, true);
+  else PQ_CACHE(128, false);
 #undef PQ_CACHE
   return pq::launch_status("pq_attn_cache_i8 launch");
 }
