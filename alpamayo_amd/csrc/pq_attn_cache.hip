@@ -649,75 +649,102 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
   }
 }
 
-// weights[b, head, j] += sum over the head's rows of exp(s_ij - lse_i).  A wave per page: its codes become matrix
-// operands once, and the rows pass 16 at a time.  Here tokens are the columns of the scores, so that the rows' sum is
-// over a lane's own values and the four groups of lanes.
+// weights[b, head, j] += sum over the head's rows of exp(s_ij - lse_i).  A unit is all rows of a sequence and head, 64 of
+// them at a time staged in LDS as operands; the waves take a segment's pages in turn, the next one's codes in flight.
+// Here tokens are the columns of the scores, so that the rows' sum is over a lane's own values and the four groups of
+// lanes, in an order of its own whatever the shares.
 template <int D, bool BF16>
-__global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheArgs a) {
-  const int lane = lane_id(), g = lane >> 4, col = lane & 15;
-  const auto cost = [&](int b) -> int64_t {
-    return span_of(a.cu, b, a.tokens).count > 0 ? static_cast<int64_t>(a.heads) * ((seq_len(a, b) + kPage - 1) / kPage) : 0;
-  };
-  const int64_t total = sum_seqs(a.batch, cost);
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-  const int64_t workers = static_cast<int64_t>(gridDim.x) * kWaves;
-  const int64_t from = w * total / workers, to = (w + 1) * total / workers;
-  for (int64_t at = from; at < to; ++at) {
-    const Found f = find_seq(a.batch, at, cost);
-    if (f.b < 0) break;
-    const Span sp = span_of(a.cu, f.b, a.tokens);
-    const int len = seq_len(a, f.b), npages = (len + kPage - 1) / kPage;
-    const int head = static_cast<int>(f.local / npages), p = static_cast<int>(f.local % npages);
-    const int rows = sp.count * a.group;
-    const int page = a.table[static_cast<int64_t>(f.b) * a.width + p];
-    if (page < 0 || page >= a.pages) continue;
-    const int64_t ph = static_cast<int64_t>(page) * a.heads + head;
-    u4 kr[4][D / 64];
+__global__ __launch_bounds__(kThreads, 2) void attn_weights_kernel(CacheArgs a) {
+  constexpr int kKs = D / 32, kChunk = 64;
+  __shared__ h8 qs[4][kKs][64];
+  __shared__ __align__(16) float cs[kChunk], zs[kChunk];
+  __shared__ __align__(16) int lims[kChunk];
+  const int t = threadIdx.x, lane = t & 63, g = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+
+  for_segments<1 << 30>(a, [&](const Segment& sg) {
+    const int* table = a.table + static_cast<int64_t>(sg.b) * a.width;
+    float* weights = a.weights + (static_cast<int64_t>(sg.b) * a.heads + sg.head) * a.span;
+    const int shift = sg.len - sg.sp.count;
+    // the first token that sees any page of the segment
+    const int seen = max(0, sg.p0 * kPage - shift);
+    for (int row0 = seen * a.group / kChunk * kChunk; row0 < sg.rows; row0 += kChunk) {
+      {
+        h8 qf[kKs];
+        float mult;
+        load_q<D, BF16>(a, sg.sp.first, sg.rows, sg.head, row0 + 16 * wave, qf, mult);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) load_k<D, false>(a.kc + ph * (kPage * D), q, kr[q]);
-    const float ks = a.ks[ph];
-    h8 kf[4][D / 32];
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) kf[q][k] = codes_f16(kr[q][k >> 1][2 * (k & 1)], kr[q][k >> 1][2 * (k & 1) + 1]);
-    float sum[4] = {0, 0, 0, 0};
-    // the first token that sees the page
-    const int seen = max(0, p * kPage - (len - sp.count));
-    for (int row0 = seen * a.group / 16 * 16; row0 < rows; row0 += 16) {
-      h8 qf[D / 32];
-      float mult;
-      load_q<D, BF16>(a, sp.first, rows, head, row0, qf, mult);
-      float c[4], z[4];
-      int limit[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = row0 + 4 * g + e, token = r / a.group;
-        c[e] = __shfl(mult, 4 * g + e) * ks;
-        limit[e] = r < rows ? token + len - sp.count + 1 : 0;
-        z[e] = 0.0f;
-        if (r < rows) z[e] = a.lse[(static_cast<int64_t>(head) * a.group + r - token * a.group) * a.tokens + sp.first + token];
-        if (z[e] == -INFINITY) limit[e] = 0;   // a row that sees nothing gives nothing
-        z[e] *= kLog2e;
-      }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f4 s = {0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[k], kf[q][k], s, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = exp2_fast(__builtin_fmaf(s[e], c[e], -z[e]));
-          sum[q] += p * kPage + 16 * q + col < limit[e] ? x : 0.0f;
+        for (int k = 0; k < kKs; ++k) qs[wave][k][lane] = qf[k];
+        if (g == 0) {
+          const int r = row0 + 16 * wave + col, token = r / a.group;
+          float z = -INFINITY;
+          if (r < sg.rows) z = a.lse[(static_cast<int64_t>(sg.head) * a.group + r - token * a.group) * a.tokens + sg.sp.first + token];
+          cs[16 * wave + col] = mult;
+          zs[16 * wave + col] = z * kLog2e;
+          lims[16 * wave + col] = z == -INFINITY ? 0 : min(token + shift + 1, sg.len);   // a row that sees nothing gives nothing
         }
       }
-    }
+      __syncthreads();
+      const int tiles = min(4, (sg.rows - row0 + 15) / 16);
+      u4 kr[4][D / 64];
+      int p = sg.p0 + wave;
+      int id = 0, id_next = 0;
+      float ks = 0.0f;
+      if (p < sg.p1) {
+        id = scalar_load(table + p);
+        if (p + kWaves < sg.p1) id_next = scalar_load(table + p + kWaves);
+        const int64_t ph = page_head(a, id, sg.head);
+        ks = scalar_load(a.ks + ph);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sum[q] = sum_xor32(sum_xor16(sum[q]));
-    const float mine = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
-    const int64_t j = static_cast<int64_t>(p) * kPage + lane;
-    if (j < len && j < a.span) a.weights[(static_cast<int64_t>(f.b) * a.heads + head) * a.span + j] += mine;
-  }
+        for (int q = 0; q < 4; ++q) load_k<D, false>(a.kc + ph * (kPage * D), q, kr[q]);
+      }
+      for (; p < sg.p1; p += kWaves) {
+        const bool there = id >= 0 && id < a.pages;
+        id = p + kWaves < sg.p1 ? id_next : id;
+        const int64_t ph = page_head(a, id, sg.head);
+        if (p + 2 * kWaves < sg.p1) id_next = scalar_load(table + p + 2 * kWaves);
+        const float ks_next = scalar_load(a.ks + ph);
+        h8 kf[4][kKs];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int k = 0; k < kKs; ++k) kf[q][k] = codes_f16(kr[q][k >> 1][2 * (k & 1)], kr[q][k >> 1][2 * (k & 1) + 1]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) load_k<D, false>(a.kc + ph * (kPage * D), q, kr[q]);
+        __builtin_amdgcn_sched_barrier(0);
+        const int64_t j = static_cast<int64_t>(p) * kPage + lane;
+        float was = 0.0f;
+        if (j < a.span) was = weights[j];
+        float sum[4] = {0, 0, 0, 0};
+        for (int i = 0; i < tiles; ++i) {
+          f4 c = *reinterpret_cast<const f4*>(cs + 16 * i + 4 * g);
+          const f4 z = *reinterpret_cast<const f4*>(zs + 16 * i + 4 * g);
+          f4 s[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) s[q] = f4{0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < kKs; ++k)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qs[i][k][lane], kf[q][k], s[q], 0, 0, 0);
+          const int4 lim = *reinterpret_cast<const int4*>(lims + 16 * i + 4 * g);
+          const int see[4] = {lim.x, lim.y, lim.z, lim.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = exp2_fast(__builtin_fmaf(s[q][e], c[e] * ks, -z[e]));
+              sum[q] += p * kPage + 16 * q + col < see[e] ? x : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum[q] = sum_xor32(sum_xor16(sum[q]));
+        const float mine = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
+        if (there && j < sg.len && j < a.span) weights[j] = was + mine;
+        ks = ks_next;
+      }
+      __syncthreads();
+    }
+  });
 }
 
 // Rows of a unit: 16 where the call's sequences have no more on the average, else 64.
@@ -816,14 +843,12 @@ extern "C" int pq_attn_cache_weights_i8(const void* q, int dtype, int64_t q_stri
   a.q_st = q_stride_token; a.q_sh = q_stride_head;
   a.batch = static_cast<int>(batch); a.width = static_cast<int>(table_width);
   a.tokens = static_cast<int>(tokens); a.heads = static_cast<int>(kv_heads); a.group = static_cast<int>(group);
-  a.pages = static_cast<int>(pages);
+  a.pages = static_cast<int>(pages); a.workers = kWorkers;
   a.scale_log2 = scale * kLog2e;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t most = (batch * kv_heads * table_width + kWaves - 1) / kWaves;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(most, 2 * kWorkers));
-  if (head_dim == 64 && dtype == PQ_BF16) attn_weights_kernel<64, true><<<grid, kThreads, 0, s>>>(a);
-  else if (head_dim == 64) attn_weights_kernel<64, false><<<grid, kThreads, 0, s>>>(a);
-  else if (dtype == PQ_BF16) attn_weights_kernel<128, true><<<grid, kThreads, 0, s>>>(a);
-  else attn_weights_kernel<128, false><<<grid, kThreads, 0, s>>>(a);
+  if (head_dim == 64 && dtype == PQ_BF16) attn_weights_kernel<64, true><<<kWorkers, kThreads, 0, s>>>(a);
+  else if (head_dim == 64) attn_weights_kernel<64, false><<<kWorkers, kThreads, 0, s>>>(a);
+  else if (dtype == PQ_BF16) attn_weights_kernel<128, true><<<kWorkers, kThreads, 0, s>>>(a);
+  else attn_weights_kernel<128, false><<<kWorkers, kThreads, 0, s>>>(a);
   return pq::launch_status("pq_attn_cache_weights_i8 launch");
 }
