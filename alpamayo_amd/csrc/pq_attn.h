@@ -90,6 +90,19 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x) {
   x += dpp_or_0<0x143, 0xc>(x);   // row_bcast:31
   return x;
 }
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROW_MASK, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += dpp_or_0<0x111, 0xf>(x);
+  x += dpp_or_0<0x112, 0xf>(x);
+  x += dpp_or_0<0x114, 0xf>(x);
+  x += dpp_or_0<0x118, 0xf>(x);
+  x += dpp_or_0<0x142, 0xa>(x);
+  x += dpp_or_0<0x143, 0xc>(x);
+  return x;
+}
 __device__ __forceinline__ int64_t read_lane(int64_t x, int lane) {
   const u2 w = __builtin_bit_cast(u2, x);
   const u2 r = {static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(w[0]), lane)),

@@ -5,10 +5,10 @@
 //
 // Two kernels.  The first picks: one workgroup per sequence and head finds
 // the smallest kept weight digit by digit (weights as unsigned keys of the
-// same order, digits of 11, 11 and 10 bits, a histogram each), then walks the
-// tokens once and writes the kept positions in order.  The second moves: one
-// workgroup per new page, head and side gathers its 64 tokens and rounds them
-// to the new page's scale, absmax / 127 of the values that they stand for.
+// same order, digits of 11, 11 and 10 bits, a histogram each), then goes over
+// the tokens once and writes the kept positions in order.  The second moves: one
+// workgroup per new page and head gathers its 64 tokens and rounds them to the
+// new page's scales, absmax / 127 of the values that they stand for.
 #include "pq_attn.h"
 
 namespace {
@@ -18,6 +18,8 @@ using namespace pqa;
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / 64;
 constexpr int kBins = 2048;
+constexpr int kOwn = 16;                        // weights of a thread, in a block of
+constexpr int kBlock = kPickThreads * kOwn;
 constexpr int kMoveThreads = 256;
 
 // Unsigned keys in the order of the weights; NaN lowest, -0 as 0.
@@ -37,11 +39,29 @@ struct PickArgs {
   int64_t span;
 };
 
+// Sum of x over the threads before this one (and, in `all`, over all of them).
+__device__ __forceinline__ uint32_t block_before(uint32_t x, uint32_t (&sums)[kPickWaves], uint32_t& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t incl = wave_scan(x);
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  uint32_t before = incl - x;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < kPickWaves; ++i) {
+    const uint32_t c = sums[i];
+    before += i < wave ? c : 0;
+    all += c;
+  }
+  __syncthreads();
+  return before;
+}
+
 __global__ __launch_bounds__(kPickThreads) void kv_pick_kernel(PickArgs a) {
   __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t above[kPickWaves];
+  __shared__ uint32_t sums[kPickWaves];
   __shared__ uint32_t chosen, rest;
-  const int b = blockIdx.y, head = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int b = blockIdx.y, head = blockIdx.x, t = threadIdx.x;
   const int64_t row = static_cast<int64_t>(b) * a.heads + head;
   const float* w = a.weights + row * a.span;
   float* wo = a.weights_out + row * a.span;
@@ -52,7 +72,27 @@ __global__ __launch_bounds__(kPickThreads) void kv_pick_kernel(PickArgs a) {
   const int len = static_cast<int>(a.lens[b] < 0 ? 0 : a.lens[b] < most ? a.lens[b] : most);
   const int left = len < a.keep ? len : a.keep;
   const int fixed = len > a.recent ? len - a.recent : 0;   // tokens from here on stay
-  int need = left - (len - fixed);                         // how many of those before them do
+  const int need = left - (len - fixed);                   // how many of those before them do
+
+  // A thread holds kOwn neighbouring weights of a block; a row of one block is read once.
+  float x[kOwn];
+  const bool quads = (a.span & 3) == 0 && (reinterpret_cast<uintptr_t>(a.weights) & 15) == 0;
+  const auto load = [&](int base) {
+    const int first = base + t * kOwn;
+#pragma unroll
+    for (int q = 0; q < kOwn; q += 4) {
+      if (quads && first + q + 4 <= len) {
+        const f4 v = *reinterpret_cast<const f4*>(w + first + q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[q + e] = v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[q + e] = first + q + e < len ? w[first + q + e] : 0.0f;
+      }
+    }
+  };
+  const bool one = len <= kBlock;
+  if (one) load(0);
 
   // the smallest kept key, and how many tokens that have it are kept
   uint32_t key = 0, quota = 0;
@@ -64,23 +104,19 @@ __global__ __launch_bounds__(kPickThreads) void kv_pick_kernel(PickArgs a) {
       const uint32_t bits = pass == 2 ? 1023u : 2047u;
       for (int i = t; i < kBins; i += kPickThreads) hist[i] = 0;
       __syncthreads();
-      for (int i = t; i < fixed; i += kPickThreads) {
-        const uint32_t u = weight_key(w[i]);
-        if ((u & mask) == key) atomicAdd(&hist[(u >> shift) & bits], 1u);
-      }
-      __syncthreads();
-      // bins from the top: thread t holds two, its wave's sum and those of the waves above tell how many lie over them
-      const uint32_t hi = hist[kBins - 1 - 2 * t], lo = hist[kBins - 2 - 2 * t];
-      uint32_t incl = hi + lo;
+      for (int base = 0; base < fixed; base += kBlock) {
+        if (!one) load(base);
 #pragma unroll
-      for (int s = 1; s < 64; s <<= 1) {
-        const uint32_t up = __shfl_up(incl, s);
-        if (lane >= s) incl += up;
+        for (int e = 0; e < kOwn; ++e) {
+          const uint32_t u = weight_key(x[e]);
+          if (base + t * kOwn + e < fixed && (u & mask) == key) atomicAdd(&hist[(u >> shift) & bits], 1u);
+        }
       }
-      if (lane == 63) above[wave] = incl;
       __syncthreads();
-      uint32_t over = incl - hi - lo;
-      for (int i = 0; i < wave; ++i) over += above[i];
+      // bins from the top, two a thread: the one in which the count passes what is wanted
+      const uint32_t hi = hist[kBins - 1 - 2 * t], lo = hist[kBins - 2 - 2 * t];
+      uint32_t all;
+      const uint32_t over = block_before(hi + lo, sums, all);
       if (over < want && over + hi >= want) { chosen = kBins - 1 - 2 * t; rest = want - over; }
       else if (over + hi < want && over + hi + lo >= want) { chosen = kBins - 2 - 2 * t; rest = want - over - hi; }
       __syncthreads();
@@ -91,47 +127,40 @@ __global__ __launch_bounds__(kPickThreads) void kv_pick_kernel(PickArgs a) {
     }
     quota = want;
   } else if (need > 0) {
-    need = fixed;
-    quota = static_cast<uint32_t>(fixed);   // all: every key is at least 0, and quota covers those that are 0
+    quota = static_cast<uint32_t>(fixed);   // all: every key is at least 0, and the quota covers those that are 0
   }
 
   // the kept tokens in order
   uint32_t ties = 0, done = 0;
-  for (int base = 0; base < len; base += kPickThreads) {
-    const int i = base + t;
-    const float x = i < len ? w[i] : 0.0f;
-    const uint32_t u = weight_key(x);
-    const bool tie = need > 0 && i < fixed && u == key;
-    const uint64_t tm = __ballot(tie);
-    const uint64_t below = (1ull << lane) - 1;
-    if (lane == 0) above[wave] = static_cast<uint32_t>(__builtin_popcountll(tm));
-    __syncthreads();
-    uint32_t tb = ties, tsum = 0;
-    for (int q = 0; q < kPickWaves; ++q) {
-      const uint32_t c = above[q];
-      if (q < wave) tb += c;
-      tsum += c;
+  for (int base = 0; base < len; base += kBlock) {
+    if (!one) load(base);
+    const int first = base + t * kOwn;
+    uint32_t tie = 0, keep = 0;              // a bit for each of the thread's tokens
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) {
+      const uint32_t u = weight_key(x[e]);
+      const bool there = first + e < len, free = first + e < fixed;
+      tie |= static_cast<uint32_t>(free && need > 0 && u == key) << e;
+      keep |= static_cast<uint32_t>(there && (!free || (need > 0 && u > key))) << e;
     }
-    ties += tsum;
-    tb += static_cast<uint32_t>(__builtin_popcountll(tm & below));
-    const bool keep = i < len && (i >= fixed || (need > 0 && (u > key || (tie && tb < quota))));
-    const uint64_t km = __ballot(keep);
-    __syncthreads();
-    if (lane == 0) above[wave] = static_cast<uint32_t>(__builtin_popcountll(km));
-    __syncthreads();
-    uint32_t at = done, ksum = 0;
-    for (int q = 0; q < kPickWaves; ++q) {
-      const uint32_t c = above[q];
-      if (q < wave) at += c;
-      ksum += c;
+    uint32_t all;
+    const uint32_t before = ties + block_before(__builtin_popcount(tie), sums, all);
+    ties += all;
+    uint32_t open = quota > before ? quota - before : 0;   // of equal ones the first
+    while (tie && open) {
+      keep |= tie & -tie;
+      tie &= tie - 1;
+      --open;
     }
-    done += ksum;
-    at += static_cast<uint32_t>(__builtin_popcountll(km & below));
-    if (keep) {
-      kept[at] = i;
-      wo[at] = x;
-    }
-    __syncthreads();
+    uint32_t at = done + block_before(__builtin_popcount(keep), sums, all);
+    done += all;
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e)
+      if (keep >> e & 1) {
+        kept[at] = first + e;
+        wo[at] = x[e];
+        ++at;
+      }
   }
   for (int64_t i = left + t; i < a.keep; i += kPickThreads) kept[i] = -1;
   for (int64_t i = left + t; i < a.span; i += kPickThreads) wo[i] = 0.0f;
@@ -148,91 +177,156 @@ struct MoveArgs {
   int heads, width, new_width, keep, pages, new_pages;
 };
 
+// Codes of K runs: 16 channels of a token; of V: a token for each lane, channels wave by wave.
+//
+// What bounds it is the way to the data, four reads after one another (length, kept place, page, codes), so a workgroup
+// takes K and V of its page on one way.  V comes through LDS, kStaged source pages at a time: a page's tokens are single
+// bytes of its rows, so all of it is read anyway, in 16-byte runs.
 template <int D>
 __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(MoveArgs a) {
-  __shared__ int64_t src[kPage];     // byte offset of each token's page side
-  __shared__ int slot[kPage];
-  __shared__ float mult[kPage];
-  __shared__ uint32_t top[4];
-  const int side = blockIdx.z, head = blockIdx.y, t = threadIdx.x;
+  constexpr int kStaged = 3;
+  constexpr int kOwnCodes = kPage * D / kMoveThreads;      // codes of a thread and side: 32 (d = 128) or 16
+  constexpr int kRuns = kOwnCodes / 16;
+  __shared__ int place[kPage];       // place of each token in its sequence
+  __shared__ int64_t src[kPage];     // codes of each token's page in front of it
+  __shared__ float mult[2][kPage];
+  __shared__ uint32_t top[2][4];
+  __shared__ __align__(16) int8_t stage[kStaged * kPage * D];
+  const int head = blockIdx.y, t = threadIdx.x;
   const int b = blockIdx.x / a.new_pages, j = blockIdx.x % a.new_pages;
   const int left = a.lens[b] - j * kPage;
-  if (left <= 0 || j >= a.new_width) return;
+  if (left <= 0) return;
   const int count = left < kPage ? left : kPage;
   const int page = a.new_table[static_cast<int64_t>(b) * a.new_width + j];
   if (page < 0 || page >= a.pages) return;
   if (t < kPage) {
     int64_t off = 0;
-    int s = 0;
-    float m = 0.0f;
+    int pos = 0;
+    float m[2] = {0.0f, 0.0f};
     if (t < count) {
-      const int pos = a.kept[(static_cast<int64_t>(b) * a.heads + head) * a.keep + j * kPage + t];
+      pos = a.kept[(static_cast<int64_t>(b) * a.heads + head) * a.keep + j * kPage + t];
       const int from = a.table[static_cast<int64_t>(b) * a.width + pos / kPage];
-      s = pos % kPage;
-      if (from >= 0 && from < a.pages) {
+      if (from >= 0 && from < a.pages) {   // else zeros
         const int64_t ph = static_cast<int64_t>(from) * a.heads + head;
         off = ph * (kPage * D);
-        m = a.scale[side][ph];
+        m[0] = a.scale[0][ph];
+        m[1] = a.scale[1][ph];
       }
     }
     src[t] = off;
-    slot[t] = s;
-    mult[t] = m;
+    place[t] = pos;
+    mult[0][t] = m[0];
+    mult[1][t] = m[1];
   }
   __syncthreads();
 
-  const int8_t* cache = a.cache[side];
-  constexpr int kOwn = kPage * D / kMoveThreads;           // codes of a thread: 32 (d = 128) or 16
-  float v[kOwn];
-  uint32_t big = 0;
-  // K: runs of 16 channels of a token; V: a token for each lane, channels wave by wave
-  if (side == 0) {
+  u4 kw[kRuns];
 #pragma unroll
-    for (int r = 0; r < kOwn / 16; ++r) {
-      const int q = t + r * kMoveThreads, tok = q / (D / 16), c = q % (D / 16);
-      const u4 w = *reinterpret_cast<const u4*>(cache + src[tok] + slot[tok] * D + c * 16);
+  for (int r = 0; r < kRuns; ++r) {
+    const int q = t + r * kMoveThreads, k = q / (D / 16), c = q % (D / 16);
+    kw[r] = *reinterpret_cast<const u4*>(a.cache[0] + src[k] + place[k] % kPage * D + c * 16);
+  }
+  const int tok = t & 63, d0 = t >> 6;
+  float v[kOwnCodes];
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        v[r * 16 + e] = static_cast<float>(static_cast<int8_t>(w[e >> 2] >> (8 * (e & 3)))) * mult[tok];
+  for (int r = 0; r < kOwnCodes; ++r) v[r] = 0.0f;
+  const int mine = tok < count ? place[tok] / kPage : -1, slot = place[tok] % kPage;
+  // tokens from `done` on are left; the pages of the next ones, in order and without repeats, up to kStaged
+  for (int done = 0; done < count;) {
+    int pages[kStaged], n = 0, next = done;
+    int64_t from[kStaged];
+    uint64_t open = __ballot(tok < count && tok >= done);
+#pragma unroll
+    for (int i = 0; i < kStaged; ++i) {
+      pages[i] = -1;
+      from[i] = 0;
+      if (open) {
+        const int lead = __builtin_ctzll(open);
+        pages[i] = place[lead] / kPage;
+        from[i] = src[lead];
+        const uint64_t its = __ballot(mine == pages[i]);
+        open &= ~its;
+        next = 64 - __builtin_clzll(its);
+        n = i + 1;
+      }
     }
-  } else {
-    const int tok = t & 63, d0 = t >> 6;
-    const int8_t* p = cache + src[tok] + slot[tok];
+    u4 w[kStaged][D / 64];
 #pragma unroll
-    for (int r = 0; r < kOwn; ++r) v[r] = static_cast<float>(p[(d0 + 4 * r) * kPage]) * mult[tok];
-  }
+    for (int i = 0; i < kStaged; ++i)
+      if (i < n)
 #pragma unroll
-  for (int r = 0; r < kOwn; ++r) {
-    const uint32_t m = __float_as_uint(v[r]) & 0x7fffffffu;
-    big = m < 0x7f800000u && m > big ? m : big;
+        for (int q = 0; q < D / 64; ++q)
+          w[i][q] = *reinterpret_cast<const u4*>(a.cache[1] + from[i] + (q * kMoveThreads + t) * 16);
+#pragma unroll
+    for (int i = 0; i < kStaged; ++i)
+      if (i < n)
+#pragma unroll
+        for (int q = 0; q < D / 64; ++q)
+          *reinterpret_cast<u4*>(stage + i * (kPage * D) + (q * kMoveThreads + t) * 16) = w[i][q];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kStaged; ++i)
+      if (mine >= 0 && mine == pages[i]) {
+#pragma unroll
+        for (int r = 0; r < kOwnCodes; ++r)
+          v[r] = static_cast<float>(stage[i * (kPage * D) + (d0 + 4 * r) * kPage + slot]) * mult[1][tok];
+      }
+    __syncthreads();
+    done = next;
   }
-  big = pq_wave_umax(big);
-  if ((t & 63) == 0) top[t >> 6] = big;
+
+  const auto magnitude = [](float x) {
+    const uint32_t m = __float_as_uint(x) & 0x7fffffffu;
+    return m < 0x7f800000u ? m : 0u;
+  };
+  uint32_t big[2] = {0, 0};
+  float x[kOwnCodes];
+#pragma unroll
+  for (int r = 0; r < kOwnCodes; ++r) {
+    const int k = (t + r / 16 * kMoveThreads) / (D / 16);
+    x[r] = static_cast<float>(static_cast<int8_t>(kw[r / 16][(r % 16) >> 2] >> (8 * (r & 3)))) * mult[0][k];
+    big[0] = max(big[0], magnitude(x[r]));
+    big[1] = max(big[1], magnitude(v[r]));
+  }
+  pq_wave_umax_n(big);
+  if ((t & 63) == 0) {
+    top[0][t >> 6] = big[0];
+    top[1][t >> 6] = big[1];
+  }
   __syncthreads();
-  const float amax = __uint_as_float(max(max(top[0], top[1]), max(top[2], top[3])));
-  const float now = amax < kTiny ? 0.0f : amax / 127.0f;
-  const float inv = now > 0.0f ? 1.0f / now : 0.0f;
   const int64_t ph = static_cast<int64_t>(page) * a.heads + head;
-  int8_t* out = a.cache[side] + ph * (kPage * D);
-  if (side == 0) {
+  float now[2], inv[2];
 #pragma unroll
-    for (int r = 0; r < kOwn / 16; ++r) {
-      const int q = t + r * kMoveThreads, tok = q / (D / 16), c = q % (D / 16);
-      if (tok >= count) continue;
-      u4 w = {0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        w[e >> 2] |= (static_cast<uint32_t>(code_of(v[r * 16 + e], inv)) & 0xffu) << (8 * (e & 3));
-      *reinterpret_cast<u4*>(out + tok * D + c * 16) = w;
-    }
-  } else {
-    const int tok = t & 63, d0 = t >> 6;
-    if (tok < count) {
-#pragma unroll
-      for (int r = 0; r < kOwn; ++r) out[(d0 + 4 * r) * kPage + tok] = static_cast<int8_t>(code_of(v[r], inv));
-    }
+  for (int s = 0; s < 2; ++s) {
+    const float amax = __uint_as_float(max(max(top[s][0], top[s][1]), max(top[s][2], top[s][3])));
+    now[s] = amax < kTiny ? 0.0f : amax / 127.0f;
+    inv[s] = now[s] > 0.0f ? 1.0f / now[s] : 0.0f;
   }
-  if (t == 0) a.scale[side][ph] = now;
+  int8_t* out = a.cache[0] + ph * (kPage * D);
+#pragma unroll
+  for (int r = 0; r < kRuns; ++r) {
+    const int q = t + r * kMoveThreads, k = q / (D / 16), c = q % (D / 16);
+    if (k >= count) continue;
+    u4 w = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      w[e >> 2] |= (static_cast<uint32_t>(code_of(x[r * 16 + e], inv[0])) & 0xffu) << (8 * (e & 3));
+    *reinterpret_cast<u4*>(out + k * D + c * 16) = w;
+  }
+  out = a.cache[1] + ph * (kPage * D);
+  if (count == kPage) {
+#pragma unroll
+    for (int r = 0; r < kOwnCodes; ++r) stage[(d0 + 4 * r) * kPage + tok] = static_cast<int8_t>(code_of(v[r], inv[1]));
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < D / 64; ++q)
+      *reinterpret_cast<u4*>(out + (q * kMoveThreads + t) * 16) = *reinterpret_cast<const u4*>(stage + (q * kMoveThreads + t) * 16);
+  } else if (tok < count) {
+#pragma unroll
+    for (int r = 0; r < kOwnCodes; ++r) out[(d0 + 4 * r) * kPage + tok] = static_cast<int8_t>(code_of(v[r], inv[1]));
+  }
+  if (t == 0) a.scale[0][ph] = now[0];
+  if (t == 1) a.scale[1][ph] = now[1];
 }
 
 }  // namespace
@@ -279,7 +373,7 @@ extern "C" int pq_kv_evict_i8(int8_t* k_cache, int8_t* v_cache, float* k_scale, 
     m.new_width = static_cast<int>(new_width); m.keep = static_cast<int>(keep);
     m.pages = static_cast<int>(pages);
     m.new_pages = static_cast<int>(new_pages < new_width ? new_pages : new_width);
-    const dim3 grid(static_cast<unsigned>(batch * m.new_pages), static_cast<unsigned>(heads), 2);
+    const dim3 grid(static_cast<unsigned>(batch * m.new_pages), static_cast<unsigned>(heads));
     if (m.new_pages > 0) {
       if (head_dim == 64) kv_move_kernel<64><<<grid, kMoveThreads, 0, s>>>(m);
       else kv_move_kernel<128><<<grid, kMoveThreads, 0, s>>>(m);
