@@ -12,8 +12,7 @@
 // finite values only, so one bad value does not wipe out its page: infinities
 // saturate, NaN is held as 0.
 //
-// One workgroup per touched page, head and side; no two write the same page
-// side.  Every byte of a page outside of what is written stays as it was.
+// One workgroup per touched page and head; no two write the same.  Every byte of a page outside of what is written stays as it was.
 #include "pq_attn.h"
 
 namespace {
@@ -35,22 +34,28 @@ struct AppendArgs {
 
 __device__ __forceinline__ int cached_len(const AppendArgs& a, int b) { return max(a.cached[b], 0); }
 
+// 8 values of a row as they lie: 16 bytes, 32 of float32.
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
-  if constexpr (DT == PQ_F32) {
-    const f4* q = reinterpret_cast<const f4*>(static_cast<const float*>(p) + i);
-    const f4 a = q[0], b = q[1];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
-  } else {
-    const u4 w = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = pq_raw_to_f32<DT>(w[j] & 0xffffu);
-      v[2 * j + 1] = pq_raw_to_f32<DT>(w[j] >> 16);
+struct Raw8 {
+  u4 w[DT == PQ_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    if constexpr (DT == PQ_F32) {
+      const u4* q = reinterpret_cast<const u4*>(static_cast<const float*>(p) + i);
+      w[0] = q[0];
+      w[1] = q[1];
+    } else {
+      w[0] = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(p) + i);
     }
   }
-}
+  __device__ __forceinline__ void clear() {
+    w[0] = u4{0, 0, 0, 0};
+    if constexpr (DT == PQ_F32) w[1] = w[0];
+  }
+  __device__ __forceinline__ float operator[](int j) const {
+    if constexpr (DT == PQ_F32) return __uint_as_float(w[j >> 2][j & 3]);
+    else return pq_raw_to_f32<DT>(j & 1 ? w[0][j >> 1] >> 16 : w[0][j >> 1] & 0xffffu);
+  }
+};
 
 // The bytes of a dword scaled by `ratio` and rounded.
 __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
@@ -63,15 +68,17 @@ __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
   return r;
 }
 
+// One workgroup takes both sides of its page and head: the way to the data (lengths, page, rows) is what bounds small
+// calls, and half as long for two sides on it.
 template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendArgs a) {
   constexpr int kChunks = D / 8;                        // 8 values of a row for each thread
   constexpr int kRows = kPage * kChunks / kThreads;     // neighbouring rows of a thread: 4 (d = 128) or 2
   constexpr int kPitch = kPage + 4;
-  __shared__ uint32_t top[4];
+  __shared__ uint32_t top[2][4];
   __shared__ __align__(16) uint8_t tile[D * kPitch];
 
-  const int side = blockIdx.z, head = blockIdx.y, t = threadIdx.x;
+  const int head = blockIdx.y, t = threadIdx.x;
   const Found f = find_seq(a.batch, blockIdx.x, [&](int b) -> int64_t {
     const int n = span_of(a.cu, b, a.tokens).count;
     return n > 0 ? (static_cast<int64_t>(n) + cached_len(a, b) % kPage + kPage - 1) / kPage : 0;
@@ -82,98 +89,115 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendArgs a) {
   const int64_t j = held / kPage + f.local;
   if (j >= a.width) return;
   const int page = a.table[static_cast<int64_t>(f.b) * a.width + j];
-  if (page < 0 || page >= a.pages) return;
   const int64_t first = j * kPage > held ? j * kPage : held;
   const int64_t end = (j + 1) * kPage < held + rows.count ? (j + 1) * kPage : held + rows.count;
   const int slot = static_cast<int>(first - j * kPage), count = static_cast<int>(end - first);
   const int64_t row0 = rows.first + (first - held);
 
-  const int64_t ph = static_cast<int64_t>(page) * a.heads + head;
-  int8_t* cache = a.cache[side] + ph * (kPage * D);
-  float* scale = a.scale[side] + ph;
-
   const int c = t % kChunks, r0 = t / kChunks * kRows;
-  float v[kRows][8];
-  uint32_t big = 0;
+  Raw8<DT> v[2][kRows];
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    // page slot r0 + r; outside of the new tokens it takes zeros
-    const int i = r0 + r - slot;
-    if (i >= 0 && i < count) {
-      load8<DT>(a.x[side], (row0 + i) * a.st[side] + head * a.sh[side] + c * 8, v[r]);
-    } else {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[r][q] = 0.0f;
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const uint32_t m = __float_as_uint(v[r][q]) & 0x7fffffffu;
-      big = m < 0x7f800000u && m > big ? m : big;
-    }
-  }
-  big = pq_wave_umax(big);
-  if ((t & 63) == 0) top[t >> 6] = big;
-  const float old = slot > 0 ? *scale : 0.0f;
-  __syncthreads();
-  const float amax = __uint_as_float(max(max(top[0], top[1]), max(top[2], top[3])));
-  const float fresh = amax < kTiny ? 0.0f : amax / 127.0f;
-  const bool grown = fresh > old;
-  const float now = grown ? fresh : old;
-  const float inv = now > 0.0f ? 1.0f / now : 0.0f;
-  const bool redo = grown && slot > 0;
-  const float ratio = redo ? old / now : 1.0f;
-
-  if (side == 0) {
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
+      // page slot r0 + r; outside of the new tokens it takes zeros
       const int i = r0 + r - slot;
-      if (i < 0 || i >= count) continue;
-      uint32_t w[2] = {0, 0};
-#pragma unroll
-      for (int q = 0; q < 8; ++q) w[q >> 2] |= (static_cast<uint32_t>(code_of(v[r][q], inv)) & 0xffu) << (8 * (q & 3));
-      *reinterpret_cast<uint2*>(cache + (r0 + r) * D + c * 8) = make_uint2(w[0], w[1]);
+      if (i >= 0 && i < count) v[s][r].load(a.x[s], (row0 + i) * a.st[s] + head * a.sh[s] + c * 8);
+      else v[s][r].clear();
     }
-    if (redo) {
-      for (int q = t; q < slot * D / 4; q += kThreads) {
-        uint32_t* p = reinterpret_cast<uint32_t*>(cache) + q;
-        *p = requant4(*p, ratio);
+  if (page < 0 || page >= a.pages) return;
+  const int64_t ph = static_cast<int64_t>(page) * a.heads + head;
+  float old[2] = {0.0f, 0.0f};
+  if (slot > 0) {
+    old[0] = a.scale[0][ph];
+    old[1] = a.scale[1][ph];
+  }
+  uint32_t big[2] = {0, 0};
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t m = __float_as_uint(v[s][r][q]) & 0x7fffffffu;
+        big[s] = max(big[s], m < 0x7f800000u ? m : 0u);
       }
-    }
-  } else {
+  pq_wave_umax_n(big);
+  if ((t & 63) == 0) {
+    top[0][t >> 6] = big[0];
+    top[1][t >> 6] = big[1];
+  }
+  __syncthreads();
+  float now[2], inv[2], ratio[2];
+  bool grown[2], redo[2];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      uint32_t w = 0;
+  for (int s = 0; s < 2; ++s) {
+    const float amax = __uint_as_float(max(max(top[s][0], top[s][1]), max(top[s][2], top[s][3])));
+    const float fresh = amax < kTiny ? 0.0f : amax / 127.0f;
+    grown[s] = fresh > old[s];
+    now[s] = grown[s] ? fresh : old[s];
+    inv[s] = now[s] > 0.0f ? 1.0f / now[s] : 0.0f;
+    redo[s] = grown[s] && slot > 0;
+    ratio[s] = redo[s] ? old[s] / now[s] : 1.0f;
+  }
+
+  int8_t* cache = a.cache[0] + ph * (kPage * D);
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) w |= (static_cast<uint32_t>(code_of(v[r][q], inv)) & 0xffu) << (8 * r);
-      uint8_t* p = tile + (c * 8 + q) * kPitch + r0;
-      if constexpr (kRows == 4) *reinterpret_cast<uint32_t*>(p) = w;
-      else *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w);
+  for (int r = 0; r < kRows; ++r) {
+    const int i = r0 + r - slot;
+    if (i < 0 || i >= count) continue;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int q = 0; q < 8; ++q) w[q >> 2] |= (static_cast<uint32_t>(code_of(v[0][r][q], inv[0])) & 0xffu) << (8 * (q & 3));
+    *reinterpret_cast<uint2*>(cache + (r0 + r) * D + c * 8) = make_uint2(w[0], w[1]);
+  }
+  if (redo[0]) {
+    for (int q = t; q < slot * D / 4; q += kThreads) {
+      uint32_t* p = reinterpret_cast<uint32_t*>(cache) + q;
+      *p = requant4(*p, ratio[0]);
     }
-    __syncthreads();
-    // 16 tokens of a channel at a time: new codes, held ones (rounded anew where the scale grew), and what lies behind
-    for (int q = t; q < D * 4; q += kThreads) {
-      const int d = q >> 2, t0 = (q & 3) * 16;
-      if (t0 >= slot + count || (t0 + 16 <= slot && !redo)) continue;
-      u4* p = reinterpret_cast<u4*>(cache + d * kPage + t0);
-      u4 w = {0, 0, 0, 0};
-      if (t0 < slot || t0 + 16 > slot + count) w = *p;
+  }
+
+  cache = a.cache[1] + ph * (kPage * D);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) w |= (static_cast<uint32_t>(code_of(v[1][r][q], inv[1])) & 0xffu) << (8 * r);
+    uint8_t* p = tile + (c * 8 + q) * kPitch + r0;
+    if constexpr (kRows == 4) *reinterpret_cast<uint32_t*>(p) = w;
+    else *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w);
+  }
+  __syncthreads();
+  // 16 tokens of a channel at a time: new codes, held ones (rounded anew where the scale grew), and what lies behind
+  for (int q = t; q < D * 4; q += kThreads) {
+    const int d = q >> 2, t0 = (q & 3) * 16;
+    if (t0 >= slot + count || (t0 + 16 <= slot && !redo[1])) continue;
+    u4* p = reinterpret_cast<u4*>(cache + d * kPage + t0);
+    u4 w = {0, 0, 0, 0};
+    if (t0 >= slot && t0 + 16 <= slot + count) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = *reinterpret_cast<const uint32_t*>(tile + d * kPitch + t0 + 4 * k);
+    } else {
+      w = *p;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t nw = *reinterpret_cast<const uint32_t*>(tile + d * kPitch + t0 + 4 * k);
-        const uint32_t was = redo ? requant4(w[k], ratio) : w[k];
+        const uint32_t fresh = *reinterpret_cast<const uint32_t*>(tile + d * kPitch + t0 + 4 * k);
+        const uint32_t was = redo[1] ? requant4(w[k], ratio[1]) : w[k];
         uint32_t r = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int at = t0 + 4 * k + e;
-          const uint32_t from = at < slot ? was : at < slot + count ? nw : w[k];
+          const uint32_t from = at < slot ? was : at < slot + count ? fresh : w[k];
           r |= from & (0xffu << (8 * e));
         }
         w[k] = r;
       }
-      *p = w;
     }
+    *p = w;
   }
-  if (t == 0 && (slot == 0 || grown)) *scale = now;
+  if (t == 0 && (slot == 0 || grown[0])) a.scale[0][ph] = now[0];
+  if (t == 1 && (slot == 0 || grown[1])) a.scale[1][ph] = now[1];
 }
 
 }  // namespace
@@ -212,7 +236,7 @@ extern "C" int pq_kv_append_i8(const void* k, const void* v, int dtype, int64_t 
   a.tokens = static_cast<int>(tokens); a.heads = static_cast<int>(heads); a.pages = static_cast<int>(pages);
   // pages that n tokens touch: at most n / 64 + 2, and at most n
   const int64_t most = tokens < tokens / kPage + 2 * batch ? tokens : tokens / kPage + 2 * batch;
-  const dim3 grid(static_cast<unsigned>(most), static_cast<unsigned>(heads), 2);
+  const dim3 grid(static_cast<unsigned>(most), static_cast<unsigned>(heads));
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define PQ_APPEND(DT_)                                                             \
   if (head_dim == 64) kv_append_kernel<DT_, 64><<<grid, kThreads, 0, s>>>(a);      \
