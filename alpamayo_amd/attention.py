@@ -40,6 +40,7 @@ from . import _lib
 from .ops import _DT, _DeviceGuard, _same_device, _stream
 
 PAGE = 64
+_MOST_STRIDE = 1 << 24
 _HALF = (torch.float16, torch.bfloat16)
 
 _attn_lib = torch.library.Library("paroquant_attn", "DEF")
@@ -143,41 +144,87 @@ def _scale(scale, d):
     return float(scale)
 
 
-def _ptr(t):
-    return t.data_ptr() if t.numel() else None
+# Whether tensors are what nearly every call hands over, in few operations; those that are not go through the checks
+# above, which say what is wrong or make the copy that is needed.
+
+def _plain_rows(t, on):
+    st = t.stride()
+    return len(st) == 3 and st[2] == 1 and not (st[0] | st[1]) & 7 and not t.data_ptr() & 15 and t.get_device() == on
+
+
+def _plain_index(t, on):
+    return t.dtype is torch.int32 and t.is_contiguous() and t.get_device() == on
+
+
+def _plain_pools(k_cache, v_cache, k_scale, v_scale, on):
+    s = k_cache.shape
+    if len(s) != 4 or s[2] != PAGE or not s[1]:
+        return False
+    two = (s[0], s[1])
+    return (k_cache.dtype is torch.int8 and v_cache.dtype is torch.int8 and v_cache.shape == (*two, s[3], PAGE)
+            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and k_scale.shape == two
+            and v_scale.shape == two and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k_scale.is_contiguous() and v_scale.is_contiguous() and not (k_cache.data_ptr() | v_cache.data_ptr()) & 15
+            and k_cache.get_device() == on and v_cache.get_device() == on and k_scale.get_device() == on
+            and v_scale.get_device() == on)
+
+
+def _launch(name, fn, dev, *args):
+    """One call of the library on dev's current stream."""
+    if dev.index == torch._C._cuda_getDevice():
+        st = fn(*args, _stream(dev))
+    else:
+        with _DeviceGuard(dev):
+            st = fn(*args, _stream(dev))
+    if st:
+        _lib.check(st, name)
 
 
 # ---------------------------------------------------------------------------
 # prompt_attention
 # ---------------------------------------------------------------------------
 
-def _prompt_impl(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale=None, causal=True):
+def _prompt_check(q, k, v, cu_seqlens_q, cu_seqlens_k):
     dev = q.device
-    _no_grad("prompt_attention", q, k, v)
     q = _heads3("q", q, _HALF)
     k, v = _heads3("k", k, (q.dtype,)), _heads3("v", v, (q.dtype,))
     _same_device("k", k, dev)
     _same_device("v", v, dev)
     if k.shape != v.shape:
         raise RuntimeError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    heads, d = k.size(1), k.size(2)
-    group = _group("q", q, heads, d)
+    _group("q", q, k.size(1), k.size(2))
     cq = _cu("cu_seqlens_q", cu_seqlens_q, dev)
+    ck = _index("cu_seqlens_k", cu_seqlens_k, (cq.numel(),), dev)
+    # a tile's rows are addressed by 32-bit offsets
+    k, v = (t.contiguous() if t.stride(0) > _MOST_STRIDE else t for t in (k, v))
+    return q, k, v, cq, ck
+
+
+def _prompt_impl(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale=None, causal=True):
+    dev, dt = q.device, q.dtype
+    _no_grad("prompt_attention", q, k, v)
+    qs, ks = q.shape, k.shape
     if cu_seqlens_k is None:
-        if k.size(0) != q.size(0):
-            raise RuntimeError(f"q has {q.size(0)} rows and k {k.size(0)}: give cu_seqlens_k")
-        ck = cq
-    else:
-        ck = _index("cu_seqlens_k", cu_seqlens_k, (cq.numel(),), dev)
+        if qs[:1] != ks[:1]:
+            raise RuntimeError(f"q has {tuple(qs)[:1]} rows and k {tuple(ks)[:1]}: give cu_seqlens_k")
+        cu_seqlens_k = cu_seqlens_q
+    on, heads = dev.index, ks[1] if len(ks) == 3 else 0
+    d = ks[2] if heads else 0
+    batch = cu_seqlens_q.numel() - 1
+    if not (dt in _HALF and k.dtype is dt and v.dtype is dt and d in (64, 128) and len(qs) == 3 and qs[2] == d
+            and qs[1] and not qs[1] % heads and v.shape == ks and _plain_rows(q, on) and _plain_rows(k, on)
+            and _plain_rows(v, on) and k.stride(0) <= _MOST_STRIDE and v.stride(0) <= _MOST_STRIDE
+            and _plain_index(cu_seqlens_q, on) and cu_seqlens_q.dim() == 1 and batch >= 0
+            and _plain_index(cu_seqlens_k, on) and cu_seqlens_k.shape == cu_seqlens_q.shape):
+        q, k, v, cu_seqlens_q, cu_seqlens_k = _prompt_check(q, k, v, cu_seqlens_q, cu_seqlens_k)
+        heads, d, batch = k.size(1), k.size(2), cu_seqlens_q.numel() - 1
     sc = _scale(scale, d)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((q.size(1), q.size(0)), dtype=torch.float32, device=dev)
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    with _DeviceGuard(dev):
-        st = _lib.load().pq_attn_prompt(_ptr(q), _ptr(k), _ptr(v), _DT[q.dtype], qs[0], qs[1], ks[0], ks[1], vs[0],
-                                        vs[1], cq.data_ptr(), ck.data_ptr(), _ptr(out), _ptr(lse), cq.numel() - 1,
-                                        q.size(0), k.size(0), heads, group, d, sc, bool(causal), _stream(dev))
-    _lib.check(st, "paroquant_attn::prompt_attention")
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((qs[1], qs[0]), dtype=torch.float32, device=dev)
+    a, b, c = q.stride(), k.stride(), v.stride()
+    _launch("paroquant_attn::prompt_attention", _lib.load().pq_attn_prompt, dev, q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), _DT[dt], a[0], a[1], b[0], b[1], c[0], c[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+            out.data_ptr(), lse.data_ptr(), batch, qs[0], ks[0], heads, qs[1] // heads, d, sc, bool(causal))
     return out, lse
 
 
@@ -204,25 +251,37 @@ def prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale=None, causa
 # kv_append_i8
 # ---------------------------------------------------------------------------
 
-def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, cached_lens):
+def _append_check(k, v, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, cached_lens):
     dev = k.device
-    _no_grad("kv_append_i8", k, v)
     k = _heads3("k", k, tuple(_DT))
     v = _heads3("v", v, (k.dtype,))
     _same_device("v", v, dev)
-    pages, heads, d = _pools(k_cache, v_cache, k_scale, v_scale, dev)
+    _, heads, d = _pools(k_cache, v_cache, k_scale, v_scale, dev)
     if k.shape != v.shape or k.size(1) != heads or k.size(2) != d:
         raise RuntimeError(f"k and v must be [tokens, {heads}, {d}] as the cache, got {tuple(k.shape)} and {tuple(v.shape)}")
     cu = _cu("cu_seqlens", cu_seqlens, dev)
     batch = cu.numel() - 1
-    table = _index("block_table", block_table, (batch, None), dev)
-    cached = _index("cached_lens", cached_lens, (batch,), dev)
-    ks, vs = k.stride(), v.stride()
-    with _DeviceGuard(dev):
-        st = _lib.load().pq_kv_append_i8(_ptr(k), _ptr(v), _DT[k.dtype], ks[0], ks[1], vs[0], vs[1], _ptr(k_cache),
-                                         _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(table), cu.data_ptr(),
-                                         _ptr(cached), batch, table.size(1), k.size(0), heads, d, pages, _stream(dev))
-    _lib.check(st, "paroquant_attn::kv_append_i8")
+    return k, v, _index("block_table", block_table, (batch, None), dev), cu, _index("cached_lens", cached_lens, (batch,), dev)
+
+
+def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens, cached_lens):
+    dev = k.device
+    _no_grad("kv_append_i8", k, v)
+    on, ks, cs = dev.index, k.shape, k_cache.shape
+    batch = cu_seqlens.numel() - 1
+    if not (k.dtype in _DT and v.dtype is k.dtype and len(ks) == 3 and ks[2] in (64, 128) and v.shape == ks
+            and _plain_rows(k, on) and _plain_rows(v, on) and _plain_pools(k_cache, v_cache, k_scale, v_scale, on)
+            and cs[1] == ks[1] and cs[3] == ks[2] and _plain_index(cu_seqlens, on) and cu_seqlens.dim() == 1
+            and batch >= 0 and _plain_index(cached_lens, on) and cached_lens.shape == (batch,)
+            and _plain_index(block_table, on) and block_table.dim() == 2 and block_table.size(0) == batch):
+        k, v, block_table, cu_seqlens, cached_lens = _append_check(k, v, k_cache, v_cache, k_scale, v_scale, block_table,
+                                                                   cu_seqlens, cached_lens)
+        batch = cu_seqlens.numel() - 1
+    a, b = k.stride(), v.stride()
+    _launch("paroquant_attn::kv_append_i8", _lib.load().pq_kv_append_i8, dev, k.data_ptr(), v.data_ptr(), _DT[k.dtype],
+            a[0], a[1], b[0], b[1], k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            block_table.data_ptr(), cu_seqlens.data_ptr(), cached_lens.data_ptr(), batch, block_table.size(1), ks[0], cs[1],
+            cs[3], cs[0])
 
 
 _attn_lib.impl("kv_append_i8", _append_impl, "CUDA")
@@ -248,29 +307,47 @@ def kv_append_i8(k, v, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqle
 # cache_attention_i8, cache_weights_i8
 # ---------------------------------------------------------------------------
 
+def _reader_check(q, k_cache, block_table, cu_seqlens_q, lens, dev):
+    """What reads the cache: q and its lengths, against a checked cache."""
+    q = _heads3("q", q, _HALF)
+    _group("q", q, k_cache.size(1), k_cache.size(3))
+    cu = _cu("cu_seqlens_q", cu_seqlens_q, dev)
+    batch = cu.numel() - 1
+    return q, _index("block_table", block_table, (batch, None), dev), cu, _index("lens", lens, (batch,), dev)
+
+
+def _plain_reader(q, cs, block_table, cu_seqlens_q, lens, on):
+    qs = q.shape
+    if len(qs) != 3 or qs[2] != cs[3] or not qs[1] or qs[1] % cs[1] or cu_seqlens_q.dim() != 1:
+        return False
+    batch = cu_seqlens_q.numel() - 1
+    return (q.dtype in _HALF and qs[2] in (64, 128) and _plain_rows(q, on) and _plain_index(cu_seqlens_q, on)
+            and batch >= 0 and _plain_index(lens, on) and lens.shape == (batch,) and _plain_index(block_table, on)
+            and block_table.dim() == 2 and block_table.size(0) == batch)
+
+
 def _cache_attn_impl(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens_q, lens, scale=None):
     dev = q.device
     _no_grad("cache_attention_i8", q)
-    q = _heads3("q", q, _HALF)
-    pages, heads, d = _pools(k_cache, v_cache, k_scale, v_scale, dev)
-    group = _group("q", q, heads, d)
-    cu = _cu("cu_seqlens_q", cu_seqlens_q, dev)
-    batch, tokens = cu.numel() - 1, q.size(0)
-    table = _index("block_table", block_table, (batch, None), dev)
-    ln = _index("lens", lens, (batch,), dev)
+    on, cs = dev.index, k_cache.shape
+    if not (_plain_pools(k_cache, v_cache, k_scale, v_scale, on)
+            and _plain_reader(q, cs, block_table, cu_seqlens_q, lens, on)):
+        _pools(k_cache, v_cache, k_scale, v_scale, dev)
+        q, block_table, cu_seqlens_q, lens = _reader_check(q, k_cache, block_table, cu_seqlens_q, lens, dev)
+    pages, heads, _, d = cs
+    tokens, hq, _ = q.shape
+    batch, group = cu_seqlens_q.numel() - 1, hq // heads
     sc = _scale(scale, d)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((q.size(1), tokens), dtype=torch.float32, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((hq, tokens), dtype=torch.float32, device=dev)
     lib = _lib.load()
-    need = int(lib.pq_attn_cache_i8_workspace_size(batch, tokens, group, d))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    qs = q.stride()
-    with _DeviceGuard(dev):
-        st = lib.pq_attn_cache_i8(_ptr(q), _DT[q.dtype], qs[0], qs[1], _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
-                                  _ptr(v_scale), _ptr(table), cu.data_ptr(), _ptr(ln), _ptr(out), _ptr(lse), batch,
-                                  table.size(1), tokens, heads, group, d, pages, sc,
-                                  ws.data_ptr() if ws is not None else None, need, _stream(dev))
-    _lib.check(st, "paroquant_attn::cache_attention_i8")
+    need = lib.pq_attn_cache_i8_workspace_size(batch, tokens, group, d)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    a = q.stride()
+    _launch("paroquant_attn::cache_attention_i8", lib.pq_attn_cache_i8, dev, q.data_ptr(), _DT[q.dtype], a[0], a[1],
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
+            cu_seqlens_q.data_ptr(), lens.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, block_table.size(1), tokens,
+            heads, group, d, pages, sc, ws.data_ptr(), need)
     return out, lse
 
 
@@ -295,30 +372,31 @@ def cache_attention_i8(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_se
 def _cache_weights_impl(q, k_cache, k_scale, block_table, cu_seqlens_q, lens, lse, weights, scale=None):
     dev = q.device
     _no_grad("cache_weights_i8", q, lse, weights)
-    q = _heads3("q", q, _HALF)
-    pages, heads, d = _cache_dims(k_cache)
-    _codes("k_cache", k_cache, pages, heads, PAGE, d, dev)
-    _scales("k_scale", k_scale, pages, heads, dev)
-    group = _group("q", q, heads, d)
-    cu = _cu("cu_seqlens_q", cu_seqlens_q, dev)
-    batch, tokens = cu.numel() - 1, q.size(0)
-    table = _index("block_table", block_table, (batch, None), dev)
-    ln = _index("lens", lens, (batch,), dev)
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (q.size(1), tokens):
-        raise RuntimeError(f"lse must be float32 {(q.size(1), tokens)}, got {lse.dtype} {tuple(lse.shape)}")
+    on, cs = dev.index, k_cache.shape
+    tokens, hq = q.shape[0], q.size(1) if q.dim() > 1 else 0
+    if not (len(cs) == 4 and cs[2] == PAGE and cs[1] and k_cache.dtype is torch.int8 and k_cache.is_contiguous()
+            and not k_cache.data_ptr() & 15 and k_cache.get_device() == on and k_scale.dtype is torch.float32
+            and k_scale.shape == (cs[0], cs[1]) and k_scale.is_contiguous() and k_scale.get_device() == on
+            and _plain_reader(q, cs, block_table, cu_seqlens_q, lens, on)):
+        pages, heads, d = _cache_dims(k_cache)
+        _codes("k_cache", k_cache, pages, heads, PAGE, d, dev)
+        _scales("k_scale", k_scale, pages, heads, dev)
+        q, block_table, cu_seqlens_q, lens = _reader_check(q, k_cache, block_table, cu_seqlens_q, lens, dev)
+    pages, heads, _, d = cs
+    batch = cu_seqlens_q.numel() - 1
+    if lse.dtype is not torch.float32 or lse.shape != (hq, tokens):
+        raise RuntimeError(f"lse must be float32 {(hq, tokens)}, got {lse.dtype} {tuple(lse.shape)}")
     _same_device("lse", lse, dev)
     lse = lse.contiguous()
     _check_weights(weights, batch, heads, dev)
     if not weights.is_contiguous():
         raise RuntimeError("weights must be contiguous")
     sc = _scale(scale, d)
-    qs = q.stride()
-    with _DeviceGuard(dev):
-        st = _lib.load().pq_attn_cache_weights_i8(_ptr(q), _DT[q.dtype], qs[0], qs[1], _ptr(k_cache), _ptr(k_scale),
-                                                  _ptr(table), cu.data_ptr(), _ptr(ln), _ptr(lse), _ptr(weights), batch,
-                                                  table.size(1), weights.size(2), tokens, heads, group, d, pages, sc,
-                                                  _stream(dev))
-    _lib.check(st, "paroquant_attn::cache_weights_i8")
+    a = q.stride()
+    _launch("paroquant_attn::cache_weights_i8", _lib.load().pq_attn_cache_weights_i8, dev, q.data_ptr(), _DT[q.dtype], a[0],
+            a[1], k_cache.data_ptr(), k_scale.data_ptr(), block_table.data_ptr(), cu_seqlens_q.data_ptr(), lens.data_ptr(),
+            lse.data_ptr(), weights.data_ptr(), batch, block_table.size(1), weights.size(2), tokens, heads, hq // heads, d,
+            pages, sc)
 
 
 def _check_weights(weights, batch, heads, dev):
@@ -352,23 +430,29 @@ def cache_weights_i8(q, k_cache, k_scale, block_table, cu_seqlens_q, lens, lse, 
 def _evict_impl(k_cache, v_cache, k_scale, v_scale, weights, block_table, lens, new_table, keep, recent):
     dev = k_cache.device
     _no_grad("cache_evict_i8", weights)
-    pages, heads, d = _pools(k_cache, v_cache, k_scale, v_scale, dev)
-    ln = _index("lens", lens, (None,), dev)
-    batch = ln.numel()
-    table = _index("block_table", block_table, (batch, None), dev)
-    new = _index("new_table", new_table, (batch, None), dev)
+    on, cs = dev.index, k_cache.shape
+    batch = lens.numel()
+    if not (_plain_pools(k_cache, v_cache, k_scale, v_scale, on) and cs[3] in (64, 128) and _plain_index(lens, on)
+            and lens.dim() == 1 and _plain_index(block_table, on) and _plain_index(new_table, on)
+            and block_table.dim() == 2 and new_table.dim() == 2 and block_table.size(0) == batch
+            and new_table.size(0) == batch):
+        _pools(k_cache, v_cache, k_scale, v_scale, dev)
+        lens = _index("lens", lens, (None,), dev)
+        batch = lens.numel()
+        block_table = _index("block_table", block_table, (batch, None), dev)
+        new_table = _index("new_table", new_table, (batch, None), dev)
+    pages, heads, _, d = cs
     _check_weights(weights, batch, heads, dev)
     if not 0 <= recent <= keep or keep < 1:
         raise RuntimeError(f"keep={keep} must be at least 1 and recent={recent} within 0..keep")
     w = weights.contiguous()
     out = torch.empty_like(w)
-    new_lens = torch.empty_like(ln)
+    new_lens = torch.empty_like(lens)
     kept = torch.empty((batch, heads, keep), dtype=torch.int32, device=dev)
-    with _DeviceGuard(dev):
-        st = _lib.load().pq_kv_evict_i8(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(w), _ptr(table),
-                                        _ptr(ln), _ptr(new), _ptr(out), _ptr(new_lens), _ptr(kept), batch, table.size(1),
-                                        new.size(1), w.size(2), heads, d, pages, keep, recent, _stream(dev))
-    _lib.check(st, "paroquant_attn::cache_evict_i8")
+    _launch("paroquant_attn::cache_evict_i8", _lib.load().pq_kv_evict_i8, dev, k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), w.data_ptr(), block_table.data_ptr(), lens.data_ptr(),
+            new_table.data_ptr(), out.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), batch, block_table.size(1),
+            new_table.size(1), w.size(2), heads, d, pages, keep, recent)
     return out, new_lens, kept
 
 
