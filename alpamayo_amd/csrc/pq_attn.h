@@ -70,6 +70,12 @@ __device__ __forceinline__ Span span_of(const int* cu, int b, int total) {
   return {lo, hi - lo};
 }
 
+// The same of a sequence that is the same in every lane.
+__device__ __forceinline__ Span uniform_span(const int* cu, int b, int total) {
+  const int lo = min(max(scalar_load(cu + b), 0), total), hi = min(max(scalar_load(cu + b + 1), lo), total);
+  return {lo, hi - lo};
+}
+
 struct Found { int b; int64_t local; };   // b < 0: past the last one
 
 // x of the lanes that the DPP control takes it from, 0 where there is none.
@@ -122,7 +128,7 @@ __device__ __forceinline__ Found find_seq(int batch, int64_t idx, F cost) {
     const int64_t incl = wave_scan(own);
     const uint64_t past = __ballot(idx < before + incl);
     if (past) {
-      const int at = __builtin_ctzll(past);
+      const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
       return {base + at, idx - before - read_lane(incl - own, at)};
     }
     before += read_lane(incl, 63);

@@ -246,8 +246,8 @@ __device__ __forceinline__ void for_segments(const CacheArgs& a, F f) {
     if (fd.b < 0) break;
     Segment s;
     s.b = fd.b;
-    s.sp = span_of(a.cu, fd.b, a.tokens);
-    s.len = seq_len(a, fd.b);
+    s.sp = uniform_span(a.cu, fd.b, a.tokens);
+    s.len = min(max(scalar_load(a.lens + fd.b), 0), a.width * kPage);
     s.npages = (s.len + kPage - 1) / kPage;
     s.rows = s.sp.count * a.group;
     const int64_t size = P::size(s.npages);

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
     }
     return;
   }
-  const Span sq = span_of(a.cu_q, f.b, a.tokens_q), sk = span_of(a.cu_k, f.b, a.tokens_k);
+  const Span sq = uniform_span(a.cu_q, f.b, a.tokens_q), sk = uniform_span(a.cu_k, f.b, a.tokens_k);
   const int rows = sq.count * a.group, row0 = static_cast<int>(f.local) * kRows, shift = sk.count - sq.count;
   // keys that a row of token i sees
   const auto sees = [&](int i) { return a.causal ? max(0, min(i + shift + 1, sk.count)) : sk.count; };
@@ -134,10 +134,11 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
   const bool valid = row < rows;
   const int token = valid ? row / a.group : 0, h = valid ? row - token * a.group : 0;
   const int limit = valid ? sees(token) : 0;
-  const int end = sees((min(row0 + kRows, rows) - 1) / a.group);
+  const auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int end = uniform(sees((min(row0 + kRows, rows) - 1) / a.group));
   const int wrow = row0 + wave * 32;
-  const int wend = wrow < rows ? sees((min(wrow + 32, rows) - 1) / a.group) : 0;   // keys that the wave's rows see
-  const int sure = wrow < rows ? sees(wrow / a.group) : 0;                         // that all of them see
+  const int wend = uniform(wrow < rows ? sees((min(wrow + 32, rows) - 1) / a.group) : 0);   // keys that the wave's rows see
+  const int sure = uniform(wrow < rows ? sees(wrow / a.group) : 0);                         // that all of them see
 
   s8 qf[kSteps];
   {
@@ -157,10 +158,10 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
   float m = -INFINITY, l = 0.0f;
   const float c = a.scale_log2;
 
-  // K: the lane's row of S^T is key kr (bits 2 and 3 of the row swapped), chunk 2 s + half in step s
-  const int kr = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;
+  // K: the lane's row of S^T is key key_row (bits 2 and 3 of the row swapped), chunk 2 s + half in step s
+  const int key_row = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;
   // V: the lane's address in a transposing read of 4 keys by 16 channels
-  const int l16 = lane & 15, vsub = lane >> 4 & 1;
+  const int vsub = lane >> 4 & 1;
 
   // the last tile's rows end with the sequence
   const int64_t kstep = kKeys * a.k_st, vstep = kKeys * a.v_st;
@@ -180,6 +181,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
   // One tile of keys.  MASKED: some rows of the wave do not see some of its keys.
   const auto tile = [&](auto mask, int k0, const uint16_t* ks, const uint16_t* vs) {
     constexpr bool kMasked = decltype(mask)::value;
+    // masked tiles are few: their LDS addresses are worked out on the spot instead of held in registers all along
+    int kr = key_row, l16 = lane & 15;
+    if constexpr (kMasked) asm volatile("" : "+v"(kr), "+v"(l16));
     f16v s[2] = {f16v{}, f16v{}};
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
@@ -228,8 +232,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
     }
     l += sum;
 
-    // In a masked tile a value that is not finite must not meet the weight 0 of a row that does not see its key:
-    // there it takes no part in the product and is added to the rows that do see it.
+    // In a masked tile a value that is not finite must not meet the weight 0 of a row that does not see its key: it takes
+    // no part in the product and is added to the rows that do see it.
     uint32_t odd = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -245,20 +249,20 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
         }
         u4 vf = {w[0][0], w[0][1], w[1][0], w[1][1]};
         if constexpr (kMasked) {
+          // a magnitude from infinity's on reaches the sign bit when this is added
+          constexpr uint32_t kPast = BF16 ? 0x00800080u : 0x04000400u;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
-            const uint32_t bad = ((vf[e] & kInf) == kInf ? 0xffffu : 0) | ((vf[e] >> 16 & kInf) == kInf ? 0xffff0000u : 0);
+            const uint32_t bad = ((vf[e] & 0x7fff7fffu) + kPast) & 0x80008000u;
             odd |= bad;
-            vf[e] &= ~bad;
+            vf[e] &= ~((bad - (bad >> 15)) | bad);
           }
         }
         o[i] = mfma32<BF16>(__builtin_bit_cast(s8, vf), pf[u], o[i]);
       }
     if constexpr (kMasked) {
       if (__any(odd != 0)) {
-        for (int key = 0; key < kKeys && k0 + key < sk.count; ++key) {
-          if (k0 + key >= limit) continue;
+        for (int key = 0; key < kKeys && k0 + key < limit; ++key)
 #pragma unroll
           for (int i = 0; i < kDt; ++i)
 #pragma unroll
@@ -267,20 +271,29 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
               const float x = pq_raw_to_f32<BF16 ? PQ_BF16 : PQ_F16>(vs[key * D + (((d >> 3) ^ swz<D>(key)) << 3) + (d & 7)]);
               if (!(fabsf(x) < INFINITY)) o[i][e] += x;
             }
-        }
       }
     }
   };
 
   if (end > 0) stage(0, 0);
-  for (int k0 = 0; k0 < end; k0 += kKeys) {
+  const auto step = [&](int k0, int at) {
     // this stage's copies are done, and no wave reads the other one any more: the next tile's go there
     pqd::wait_vmcnt<0>();
     __syncthreads();
-    const int at = k0 / kKeys & 1;
     if (k0 + kKeys < end) stage(k0 + kKeys, at ^ 1);
-    if (k0 + kKeys <= sure) tile(std::false_type{}, k0, lds[at][0], lds[at][1]);
-    else if (k0 < wend) tile(std::true_type{}, k0, lds[at][0], lds[at][1]);
+  };
+  // tiles that every row of the wave sees whole, the two stages in turn by their own code
+  int k0 = 0;
+  for (; k0 + 2 * kKeys <= sure; k0 += 2 * kKeys) {
+    step(k0, 0);
+    tile(std::false_type{}, k0, lds[0][0], lds[0][1]);
+    step(k0 + kKeys, 1);
+    tile(std::false_type{}, k0 + kKeys, lds[1][0], lds[1][1]);
+  }
+  for (; k0 < end; k0 += kKeys) {
+    const int at = k0 / kKeys & 1;
+    step(k0, at);
+    if (k0 < wend) tile(std::true_type{}, k0, lds[at][0], lds[at][1]);
   }
 
   l = sum_xor32(l);
