@@ -88,7 +88,9 @@ SIGNATURES = {
     "pq_w4a16_linear_workspace_size": (_SZ, [_I64, _I64]),
     "pq_w4a16_linear": (_INT, [_P, _INT, _P, _P, _P, _P, _P, _P, _INT, _P, _INT, _I64, _I64, _I64, _INT, _UINT, _P,
                                _SZ, _P]),
-    "pq_attn_prompt": (_INT, [_P, _P, _P, _INT, *[_I64] * 6, _P, _P, _P, _P, *[_I64] * 6, _F, _INT, _P]),
+    "pq_attn_prompt": (_INT, [_P, _P, _P, _INT, *[_I64] * 6, _P, _P, _P, _P, *[_I64] * 6, _F, _INT, _P, _SZ,
+                              _P]),
+    "pq_attn_prompt_workspace_size": (_SZ, [_I64] * 6),
     "pq_kv_append_i8": (_INT, [_P, _P, _INT, *[_I64] * 4, *[_P] * 7, *[_I64] * 6, _P]),
     "pq_attn_cache_i8_workspace_size": (_SZ, [_I64] * 4),
     "pq_attn_cache_i8": (_INT, [_P, _INT, _I64, _I64, *[_P] * 9, *[_I64] * 7, _F, _P, _SZ, _P]),

@@ -221,10 +221,14 @@ def _prompt_impl(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale=None, causal=Tr
     sc = _scale(scale, d)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((qs[1], qs[0]), dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    need = lib.pq_attn_prompt_workspace_size(batch, qs[0], ks[0], heads, qs[1] // heads, d)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     a, b, c = q.stride(), k.stride(), v.stride()
-    _launch("paroquant_attn::prompt_attention", _lib.load().pq_attn_prompt, dev, q.data_ptr(), k.data_ptr(),
+    _launch("paroquant_attn::prompt_attention", lib.pq_attn_prompt, dev, q.data_ptr(), k.data_ptr(),
             v.data_ptr(), _DT[dt], a[0], a[1], b[0], b[1], c[0], c[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-            out.data_ptr(), lse.data_ptr(), batch, qs[0], ks[0], heads, qs[1] // heads, d, sc, bool(causal))
+            out.data_ptr(), lse.data_ptr(), batch, qs[0], ks[0], heads, qs[1] // heads, d, sc, bool(causal),
+            ws.data_ptr() if need else None, need)
     return out, lse
 
 

@@ -43,7 +43,8 @@ struct PromptArgs {
   const int* cu_q;           // [batch + 1]
   const int* cu_k;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
-  int batch, tokens_q, tokens_k, heads, group, tiles, causal;
+  float* part;               // partial results of a call whose keys are split
+  int batch, tokens_q, tokens_k, heads, group, tiles, causal, parts;
   float scale_log2;
 };
 
@@ -99,6 +100,68 @@ struct Chunks {
   }
 };
 
+// Row tiles of a sequence of n queries and m keys, and those of them that have more than c key tiles to go through.
+__device__ __forceinline__ uint32_t tiles_of(const PromptArgs& a, int n) {
+  return (static_cast<uint32_t>(n) * a.group + kRows - 1) / kRows;
+}
+__device__ __forceinline__ uint32_t tiles_over(const PromptArgs& a, int n, int m, int c) {
+  if (c < 0) return tiles_of(a, n);
+  if (!a.causal) return m > c * kKeys ? tiles_of(a, n) : 0;
+  // the first `few` tokens see c key tiles or less; only the last row tile may end inside of kRows rows
+  const int few = static_cast<int>(min(max(static_cast<int64_t>(c) * kKeys - (m - n), static_cast<int64_t>(0)), static_cast<int64_t>(n)));
+  return few == n ? 0 : tiles_of(a, n) - static_cast<uint32_t>(few) * a.group / kRows;
+}
+
+// The row tile of this rank when those with most key tiles come first: sequence and tile in it.  The longest ones start
+// first, and what starts together is about as long.  Found by halving the range of key tiles, every lane counting for
+// sequences of its own.
+__device__ __forceinline__ Found find_tile(const PromptArgs& a, int rank) {
+  if (a.batch == 1) {
+    const int all = tiles_of(a, uniform_span(a.cu_q, 0, a.tokens_q).count);
+    return rank < all ? Found{0, all - 1 - rank} : Found{-1, rank - all};
+  }
+  const int lane = lane_id();
+  const auto lens = [&](int b, int& n, int& m) {
+    n = b < a.batch ? span_of(a.cu_q, b, a.tokens_q).count : 0;
+    m = b < a.batch ? span_of(a.cu_k, b, a.tokens_k).count : 0;
+  };
+  int n0, m0;            // of the first 64 sequences, most often of all
+  lens(lane, n0, m0);
+  const auto over = [&](int c) {
+    uint32_t sum = tiles_over(a, n0, m0, c);
+    for (int b = 64 + lane; b < a.batch; b += 64) {
+      int n, m;
+      lens(b, n, m);
+      sum += tiles_over(a, n, m, c);
+    }
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan(sum)), 63));
+  };
+  const uint32_t all = over(-1), r = static_cast<uint32_t>(rank);
+  if (r >= all) return {-1, static_cast<int64_t>(r - all)};
+  int low = -1, high = (a.tokens_k + kKeys - 1) / kKeys;   // of the tile: more than low, at most high
+  while (high - low > 1) {
+    const int mid = low + (high - low) / 2;
+    if (over(mid) <= r) high = mid;
+    else low = mid;
+  }
+  // among the tiles with just that many, by sequence, late ones first
+  uint32_t before = over(high);
+  for (int base = 0; base < a.batch; base += 64) {
+    int n = n0, m = m0;
+    if (base > 0) lens(base + lane, n, m);
+    const uint32_t more = tiles_over(a, n, m, high), own = tiles_over(a, n, m, low) - more, incl = wave_scan(own);
+    const uint64_t past = __ballot(r < before + incl);
+    if (past) {
+      const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
+      const auto get = [&](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), at)); };
+      return {base + at, static_cast<int64_t>(get(tiles_of(a, n)) - get(more) - 1 - (r - before - get(incl - own)))};
+    }
+    before += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(incl), 63));
+  }
+  return {-1, 0};
+}
+
+// With a.parts > 1 a workgroup takes one of so many parts of its tile's keys and leaves a partial result.
 template <int D, bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) {
   constexpr int kDt = D / 32, kSteps = D / 16;
@@ -106,16 +169,14 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
   const int t = threadIdx.x, lane = t & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int head = blockIdx.x % a.heads;
-  const int idx = a.tiles - 1 - blockIdx.x / a.heads;   // late rows of a prompt see most keys: they start first
-
-  const Found f = find_seq(a.batch, idx, [&](int b) -> int64_t {
-    return (static_cast<int64_t>(span_of(a.cu_q, b, a.tokens_q).count) * a.group + kRows - 1) / kRows;
-  });
+  const int part = blockIdx.x / a.heads % a.parts, rank = blockIdx.x / a.heads / a.parts;
+  const Found f = find_tile(a, rank);
   if (f.b < 0) {
+    if (part > 0) return;
     // the workgroups left over clear the rows outside of the sequences
     const int lo = a.batch > 0 ? min(max(a.cu_q[0], 0), a.tokens_q) : 0;
     const int hi = a.batch > 0 ? max(lo, min(max(a.cu_q[a.batch], 0), a.tokens_q)) : 0;
-    const int rest = a.tokens_q - (hi - lo), left = a.tiles - (idx - static_cast<int>(f.local));
+    const int rest = a.tokens_q - (hi - lo), left = a.tiles - (rank - static_cast<int>(f.local));
     for (int i = static_cast<int>(f.local); i < rest; i += left) {
       const int token = i < lo ? i : hi + i - lo;
       uint16_t* op = a.out + (static_cast<int64_t>(token) * a.heads + head) * a.group * D;
@@ -130,13 +191,17 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
   // keys that a row of token i sees
   const auto sees = [&](int i) { return a.causal ? max(0, min(i + shift + 1, sk.count)) : sk.count; };
 
-  const int row = row0 + wave * 32 + col;
+  const int wrow = row0 + wave * 32, row = wrow + col;
   const bool valid = row < rows;
   const int token = valid ? row / a.group : 0, h = valid ? row - token * a.group : 0;
   const int limit = valid ? sees(token) : 0;
   const auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  const int end = uniform(sees((min(row0 + kRows, rows) - 1) / a.group));
-  const int wrow = row0 + wave * 32;
+  int begin = 0, end = uniform(sees((min(row0 + kRows, rows) - 1) / a.group));
+  if (a.parts > 1) {
+    const int each = ((end + kKeys - 1) / kKeys + a.parts - 1) / a.parts * kKeys;
+    begin = min(part * each, end);
+    end = min(begin + each, end);
+  }
   const int wend = uniform(wrow < rows ? sees((min(wrow + 32, rows) - 1) / a.group) : 0);   // keys that the wave's rows see
   const int sure = uniform(wrow < rows ? sees(wrow / a.group) : 0);                         // that all of them see
 
@@ -163,18 +228,16 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
   // V: the lane's address in a transposing read of 4 keys by 16 channels
   const int vsub = lane >> 4 & 1;
 
-  // the last tile's rows end with the sequence
-  const int64_t kstep = kKeys * a.k_st, vstep = kKeys * a.v_st;
+  // asks for the tile at key k0; the last tile's rows end with the sequence
   const Chunks<D> kc(a.k_st, kKeys), vc(a.v_st, kKeys);
   const auto stage = [&](int k0, int to) {
-    const int tile = k0 / kKeys;
+    const uint16_t *kt = kb + k0 * a.k_st, *vt = vb + k0 * a.v_st;
     if (k0 + kKeys <= sk.count) {
-      kc.copy(kb + tile * kstep, lds[to][0]);
-      vc.copy(vb + tile * vstep, lds[to][1]);
+      kc.copy(kt, lds[to][0]);
+      vc.copy(vt, lds[to][1]);
     } else {
-      const Chunks<D> kl(a.k_st, sk.count - 1 - k0), vl(a.v_st, sk.count - 1 - k0);
-      kl.copy(kb + tile * kstep, lds[to][0]);
-      vl.copy(vb + tile * vstep, lds[to][1]);
+      Chunks<D>(a.k_st, sk.count - 1 - k0).copy(kt, lds[to][0]);
+      Chunks<D>(a.v_st, sk.count - 1 - k0).copy(vt, lds[to][1]);
     }
   };
 
@@ -275,7 +338,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
     }
   };
 
-  if (end > 0) stage(0, 0);
+  if (begin < end) stage(begin, 0);
   const auto step = [&](int k0, int at) {
     // this stage's copies are done, and no wave reads the other one any more: the next tile's go there
     pqd::wait_vmcnt<0>();
@@ -283,21 +346,38 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
     if (k0 + kKeys < end) stage(k0 + kKeys, at ^ 1);
   };
   // tiles that every row of the wave sees whole, the two stages in turn by their own code
-  int k0 = 0;
-  for (; k0 + 2 * kKeys <= sure; k0 += 2 * kKeys) {
+  int k0 = begin;
+  for (; k0 + 2 * kKeys <= min(sure, end); k0 += 2 * kKeys) {
     step(k0, 0);
     tile(std::false_type{}, k0, lds[0][0], lds[0][1]);
     step(k0 + kKeys, 1);
     tile(std::false_type{}, k0 + kKeys, lds[1][0], lds[1][1]);
   }
   for (; k0 < end; k0 += kKeys) {
-    const int at = k0 / kKeys & 1;
+    const int at = (k0 - begin) / kKeys & 1;
     step(k0, at);
     if (k0 < wend) tile(std::true_type{}, k0, lds[at][0], lds[at][1]);
   }
 
   l = sum_xor32(l);
   if (!valid) return;
+  if (a.parts > 1) {
+    // [part][token][head] rows of results, then of maxima, then of sums; a part without keys leaves no results
+    const int64_t all = static_cast<int64_t>(a.tokens_q) * a.heads * a.group;
+    const int64_t at = part * all + (static_cast<int64_t>(sq.first) + token) * a.heads * a.group + head * a.group + h;
+    float* const stats = a.part + a.parts * all * D;
+    if (half == 0) {
+      stats[at] = m;
+      stats[a.parts * all + at] = l;
+    }
+    if (begin < end)
+#pragma unroll
+      for (int i = 0; i < kDt; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<f4*>(a.part + at * D + 32 * i + 2 * e + 4 * half) = f4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+    return;
+  }
   const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
   uint16_t* op = a.out + ((static_cast<int64_t>(sq.first) + token) * a.heads * a.group + head * a.group + h) * D;
 #pragma unroll
@@ -310,14 +390,69 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
     a.lse[(static_cast<int64_t>(head) * a.group + h) * a.tokens_q + sq.first + token] = (m + log2_fast(l)) * kLn2;
 }
 
+// Joins the parts of a row, a wave for each.
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads) void attn_prompt_join_kernel(PromptArgs a) {
+  constexpr int kV = D / 64;
+  const int lane = lane_id(), hq = a.heads * a.group;
+  const int64_t all = static_cast<int64_t>(a.tokens_q) * hq;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  const int token = static_cast<int>(row / hq), h = static_cast<int>(row % hq);
+  // rows outside of the sequences are done
+  if (row >= all || a.batch == 0 || token < scalar_load(a.cu_q) || token >= scalar_load(a.cu_q + a.batch)) return;
+  const float* const stats = a.part + a.parts * all * D;
+  float pm = -INFINITY, pl = 0.0f;      // of part `lane`
+  if (lane < a.parts) {
+    pm = stats[lane * all + row];
+    pl = stats[(a.parts + lane) * all + row];
+  }
+  float m = pm;
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+  const float f = m == -INFINITY ? 0.0f : exp2_fast(pm - m);
+  float l = pl * f, o[kV];
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) l += __shfl_xor(l, s);
+#pragma unroll
+  for (int k = 0; k < kV; ++k) o[k] = 0.0f;
+  for (int p = 0; p < a.parts; ++p) {
+    const float c = __shfl(f, p);
+    if (c == 0.0f) continue;            // nothing, or nothing that counts
+#pragma unroll
+    for (int k = 0; k < kV; ++k) o[k] += a.part[(p * all + row) * D + lane * kV + k] * c;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+#pragma unroll
+  for (int k = 0; k < kV; ++k) {
+    const float y = o[k] * inv;
+    a.out[row * D + lane * kV + k] = BF16 ? pq_f32_to_bf16(y) : pq_f32_to_f16(y);
+  }
+  if (lane == 0) a.lse[static_cast<int64_t>(h) * a.tokens_q + token] = (m + log2_fast(l)) * kLn2;
+}
+
+// Parts of the keys for a call: as many as find room on the card (two workgroups a CU), of four key tiles or more on the
+// average (512 queries on 4101 keys 81 -> TBD us, 1024 on 1024 28 us either way).
+int parts_of(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t kv_heads, int64_t group) {
+  const int64_t wgs = (tokens_q * group / kRows + std::min(batch, tokens_q)) * kv_heads;
+  const int64_t room = 512 / std::max<int64_t>(wgs, 1), tiles = tokens_k / kKeys / std::max<int64_t>(batch, 1);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({room, tiles / 4, 64})));
+}
+
 }  // namespace
+
+extern "C" size_t pq_attn_prompt_workspace_size(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t kv_heads,
+                                                int64_t group, int64_t head_dim) {
+  if (batch <= 0 || tokens_q <= 0 || tokens_k <= 0 || kv_heads <= 0 || group <= 0 || head_dim <= 0) return 0;
+  const int parts = parts_of(batch, tokens_q, tokens_k, kv_heads, group);
+  return parts > 1 ? static_cast<size_t>(parts) * tokens_q * kv_heads * group * (head_dim + 2) * sizeof(float) : 0;
+}
 
 extern "C" int pq_attn_prompt(const void* q, const void* k, const void* v, int dtype, int64_t q_stride_token,
                               int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head,
                               int64_t v_stride_token, int64_t v_stride_head, const int32_t* cu_seqlens_q,
                               const int32_t* cu_seqlens_k, void* out, float* lse, int64_t batch, int64_t tokens_q,
                               int64_t tokens_k, int64_t kv_heads, int64_t group, int64_t head_dim, float scale,
-                              int causal, void* stream) {
+                              int causal, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "pq_attn_prompt";
   PQ_REQUIRE(dtype == PQ_F16 || dtype == PQ_BF16, PQ_ERR_UNSUPPORTED, "%s: dtype code %d (Half or BFloat16)", who, dtype);
   PQ_REQUIRE(head_dim == 64 || head_dim == 128, PQ_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 64, 128)", who,
@@ -325,7 +460,7 @@ extern "C" int pq_attn_prompt(const void* q, const void* k, const void* v, int d
   PQ_REQUIRE(kv_heads >= 1 && group >= 1 && kv_heads * group <= 65535, PQ_ERR_ARG, "%s: kv_heads=%lld group=%lld", who,
              (long long)kv_heads, (long long)group);
   PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffLL && tokens_q >= 0 && tokens_k >= 0 && tokens_k <= 0x7fffffffLL - 64 &&
-                 tokens_q * group <= 0x7fffffffLL - kRows, PQ_ERR_ARG,
+                 tokens_q * group <= 0x7fffffffLL - 128, PQ_ERR_ARG,
              "%s: batch=%lld tokens_q=%lld tokens_k=%lld", who, (long long)batch, (long long)tokens_q, (long long)tokens_k);
   PQ_REQUIRE(scale > 0.0f && scale < INFINITY, PQ_ERR_ARG, "%s: scale=%g must be positive and finite", who, scale);
   if (tokens_q == 0) return PQ_OK;
@@ -348,15 +483,28 @@ extern "C" int pq_attn_prompt(const void* q, const void* k, const void* v, int d
   a.batch = static_cast<int>(batch); a.tokens_q = static_cast<int>(tokens_q); a.tokens_k = static_cast<int>(tokens_k);
   a.heads = static_cast<int>(kv_heads); a.group = static_cast<int>(group); a.causal = causal != 0;
   a.scale_log2 = scale * kLog2e;
+  const size_t need = pq_attn_prompt_workspace_size(batch, tokens_q, tokens_k, kv_heads, group, head_dim);
+  PQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && pq::aligned_to(workspace, 16)), PQ_ERR_WORKSPACE,
+             "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", who, need,
+             workspace ? workspace_bytes : (size_t)0);
+  a.part = static_cast<float*>(workspace);
+  a.parts = need ? parts_of(batch, tokens_q, tokens_k, kv_heads, group) : 1;
   // tiles of all sequences, each of which may end inside one, and one for the rows outside of them
   const int64_t tiles = tokens_q * group / kRows + std::min<int64_t>(batch, tokens_q) + 1;
-  PQ_REQUIRE(tiles * kv_heads <= 0x7fffffffLL, PQ_ERR_ARG, "%s: too many rows", who);
+  PQ_REQUIRE(tiles * kv_heads * a.parts <= 0x7fffffffLL, PQ_ERR_ARG, "%s: too many rows", who);
   a.tiles = static_cast<int>(tiles);
-  const unsigned grid = static_cast<unsigned>(tiles * kv_heads);
+  const unsigned grid = static_cast<unsigned>(tiles * kv_heads * a.parts);
+  const unsigned join = static_cast<unsigned>((tokens_q * kv_heads * group + kWaves - 1) / kWaves);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (head_dim == 64 && dtype == PQ_BF16) attn_prompt_kernel<64, true><<<grid, kThreads, 0, s>>>(a);
-  else if (head_dim == 64) attn_prompt_kernel<64, false><<<grid, kThreads, 0, s>>>(a);
-  else if (dtype == PQ_BF16) attn_prompt_kernel<128, true><<<grid, kThreads, 0, s>>>(a);
-  else attn_prompt_kernel<128, false><<<grid, kThreads, 0, s>>>(a);
+#define PQ_PROMPT(D_, BF_)                                                                       \
+  do {                                                                                           \
+    attn_prompt_kernel<D_, BF_><<<grid, kThreads, 0, s>>>(a);                                    \
+    if (a.parts > 1) attn_prompt_join_kernel<D_, BF_><<<join, kThreads, 0, s>>>(a);              \
+  } while (0)
+  if (head_dim == 64 && dtype == PQ_BF16) PQ_PROMPT(64, true);
+  else if (head_dim == 64) PQ_PROMPT(64, false);
+  else if (dtype == PQ_BF16) PQ_PROMPT(128, true);
+  else PQ_PROMPT(128, false);
+#undef PQ_PROMPT
   return pq::launch_status("pq_attn_prompt launch");
 }

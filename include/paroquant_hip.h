@@ -463,12 +463,18 @@ int pq_w4a8_linear_group_intermediates(const void* x, const void* x2, const void
  *   out = softmax(scale * q k^T) v,  lse = log(sum exp(scale * q k^T))
  * causal != 0: query i of n sees keys j <= i + m - n of m.  Rows that see no
  * key, and rows outside of the sequences, get zeros and lse = -inf; what a
- * row does not see has no effect on it.  head_dim in {64, 128}; scale > 0. */
+ * row does not see has no effect on it.  head_dim in {64, 128}; scale > 0.
+ * workspace: pq_attn_prompt_workspace_size bytes (0 where the rows fill the
+ * card), 16-byte aligned, for the partial results of calls whose keys are
+ * split over workgroups; its content does not matter, and calls that may run
+ * at the same time must not share one. */
+size_t pq_attn_prompt_workspace_size(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t kv_heads,
+                                     int64_t group, int64_t head_dim);
 int pq_attn_prompt(const void* q, const void* k, const void* v, int dtype, int64_t q_stride_token,
                    int64_t q_stride_head, int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token,
                    int64_t v_stride_head, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* out,
                    float* lse, int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t kv_heads, int64_t group,
-                   int64_t head_dim, float scale, int causal, void* stream);
+                   int64_t head_dim, float scale, int causal, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The paged int8 cache of the entry points below: k_cache int8 [pages, heads,
  * 64, head_dim], v_cache int8 [pages, heads, head_dim, 64], k_scale and

@@ -99,6 +99,15 @@ def test_prompt_other_key_lengths(lens_q, lens_k, causal):
     _prompt_case(lens_q, lens_k, 4, 2, 128, BF, causal=causal, seed=3)
 
 
+@pytest.mark.parametrize("d,dtype", [(64, BF), (128, HF)])
+@pytest.mark.parametrize("lens_q,lens_k", [([5], [3000]), ([130, 1], [1990, 4003]), ([64, 0, 3], [2500, 700, 2600]), ([900], [900])])
+def test_prompt_keys_split_over_workgroups(lens_q, lens_k, d, dtype):
+    """Few rows on many keys: parts of the keys, joined; some rows see nothing of the later parts."""
+    need = attention._lib.load().pq_attn_prompt_workspace_size(len(lens_q), sum(lens_q) + 2, sum(lens_k) + 2, 2, 2, d)
+    assert need > 0, "the case is meant to be split"
+    _prompt_case(lens_q, lens_k, 4, 2, d, dtype, tail=2, seed=sum(lens_q))
+
+
 def test_prompt_rows_outside_sequences():
     _prompt_case([40, 30], [40, 30], 4, 2, 128, BF, tail=37, seed=5)
     _prompt_case([0], [0], 4, 2, 64, HF, tail=200, seed=5)
