@@ -301,8 +301,8 @@ def kv_append_i8(k, v, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqle
 
     A page's scale for a head is the absmax of what it holds / 127, a code round(x / scale).  Where new tokens are larger
     than what their page holds, its codes are rounded to the new scale; a page whose first token is new starts afresh.
-    NaN is held as 0, infinities as the largest code.  The lengths are the caller's to advance.  A page may belong to
-    one sequence of the call only."""
+    NaN is held as 0, infinities as the largest code.  The lengths are the caller's to advance.  A page that is
+    written to may belong to one sequence of the call only; pages in front of it may be shared."""
     torch.ops.paroquant_attn.kv_append_i8.default(k, v, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens,
                                                   cached_lens)
 
@@ -377,7 +377,7 @@ def _cache_weights_impl(q, k_cache, k_scale, block_table, cu_seqlens_q, lens, ls
     dev = q.device
     _no_grad("cache_weights_i8", q, lse, weights)
     on, cs = dev.index, k_cache.shape
-    tokens, hq = q.shape[0], q.size(1) if q.dim() > 1 else 0
+    hq, tokens = (q.size(1), q.size(0)) if q.dim() == 3 else (0, 0)
     if not (len(cs) == 4 and cs[2] == PAGE and cs[1] and k_cache.dtype is torch.int8 and k_cache.is_contiguous()
             and not k_cache.data_ptr() & 15 and k_cache.get_device() == on and k_scale.dtype is torch.float32
             and k_scale.shape == (cs[0], cs[1]) and k_scale.is_contiguous() and k_scale.get_device() == on

@@ -159,9 +159,9 @@ __device__ __forceinline__ h8 codes_f16(uint32_t lo, uint32_t hi) {
 }
 
 __device__ __forceinline__ int code_of(float x, float inv) {
-  // NaN holds the place of a zero; infinities saturate
+  // NaN holds the place of a zero (an infinity of a page without a scale too); infinities saturate
   const float r = __builtin_rintf(x * inv);
-  return x != x ? 0 : static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
+  return r != r ? 0 : static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
 }
 
 }  // namespace pqa

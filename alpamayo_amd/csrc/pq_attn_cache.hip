@@ -361,6 +361,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_cache_kernel(CacheArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         h8 pf[2];
         rw.weigh(s, ks, !there || (p + 1) * kPage > rw.sure, (there ? rw.limit : 0) - p * kPage, pf);
+        if (!there) vs = 0.0f;   // the scale of the page read in its place may be anything
 #pragma unroll
         for (int k = 0; k < kDt; ++k) rw.add(k, codes_f16(vr[k][0], vr[k][1]), codes_f16(vr[k][2], vr[k][3]), pf, vs);
         load_v(ph);
@@ -479,6 +480,7 @@ __global__ __launch_bounds__(kThreads, 2) void attn_cache_rows_kernel(CacheArgs 
             s[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[from][q][k][lane], rw.qf[k], s[q], 0, 0, 0);
         h8 pf[2];
         rw.weigh(s, ks, !there || (p + 1) * kPage > rw.sure, (there ? rw.limit : 0) - p * kPage, pf);
+        if (!there) vs = 0.0f;   // the scale of the page read in its place may be anything
 #pragma unroll
         for (int k = 0; k < kDt; ++k) rw.add(k, vf[from][k][0][lane], vf[from][k][1][lane], pf, vs);
       }
@@ -755,7 +757,7 @@ int check(const char* who, const void* q, int dtype, int64_t q_st, int64_t q_sh,
           int64_t heads, int64_t group, int64_t d, int64_t pages, float scale) {
   PQ_REQUIRE(dtype == PQ_F16 || dtype == PQ_BF16, PQ_ERR_UNSUPPORTED, "%s: dtype code %d (Half or BFloat16)", who, dtype);
   PQ_REQUIRE(d == 64 || d == 128, PQ_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 64, 128)", who, (long long)d);
-  PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffffLL && width >= 0 && width <= 0x7fffffffLL / kPage, PQ_ERR_ARG,
+  PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffLL && width >= 0 && width <= 0x7fffffffLL / kPage, PQ_ERR_ARG,
              "%s: batch=%lld table_width=%lld", who, (long long)batch, (long long)width);
   PQ_REQUIRE(heads >= 1 && group >= 1 && heads * group <= 65535, PQ_ERR_ARG, "%s: kv_heads=%lld group=%lld", who,
              (long long)heads, (long long)group);

@@ -187,6 +187,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
     return;
   }
   const Span sq = uniform_span(a.cu_q, f.b, a.tokens_q), sk = uniform_span(a.cu_k, f.b, a.tokens_k);
+  // offsets that do not ascend can make more tiles than 32 bits count
+  if (f.local < 0 || f.local >= tiles_of(a, sq.count)) return;
   const int rows = sq.count * a.group, row0 = static_cast<int>(f.local) * kRows, shift = sk.count - sq.count;
   // keys that a row of token i sees
   const auto sees = [&](int i) { return a.causal ? max(0, min(i + shift + 1, sk.count)) : sk.count; };

@@ -212,7 +212,7 @@ extern "C" int pq_kv_append_i8(const void* k, const void* v, int dtype, int64_t 
              "%s: dtype code %d (Float, Half or BFloat16)", who, dtype);
   PQ_REQUIRE(head_dim == 64 || head_dim == 128, PQ_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 64, 128)", who,
              (long long)head_dim);
-  PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffffLL && table_width >= 0 && table_width <= 0x7fffffffLL / kPage, PQ_ERR_ARG,
+  PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffLL && table_width >= 0 && table_width <= 0x7fffffffLL / kPage, PQ_ERR_ARG,
              "%s: batch=%lld table_width=%lld", who, (long long)batch, (long long)table_width);
   PQ_REQUIRE(tokens >= 0 && tokens <= 0x7fffffffLL && pages >= 0 && pages <= 0x7fffffffLL, PQ_ERR_ARG,
              "%s: tokens=%lld pages=%lld", who, (long long)tokens, (long long)pages);

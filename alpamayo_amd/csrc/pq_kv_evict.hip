@@ -343,7 +343,7 @@ extern "C" int pq_kv_evict_i8(int8_t* k_cache, int8_t* v_cache, float* k_scale, 
              "%s: batch=%lld heads=%lld (at most 65535)", who, (long long)batch, (long long)heads);
   PQ_REQUIRE(table_width >= 0 && table_width <= 0x7fffffffLL / kPage && new_width >= 0 &&
                  new_width <= 0x7fffffffLL / kPage && pages >= 0 && pages <= 0x7fffffffLL && span >= 0 &&
-                 span <= 0x7fffffffLL, PQ_ERR_ARG,
+                 span <= 0x40000000LL, PQ_ERR_ARG,
              "%s: table_width=%lld new_width=%lld pages=%lld span=%lld", who, (long long)table_width,
              (long long)new_width, (long long)pages, (long long)span);
   PQ_REQUIRE(keep >= 1 && keep <= 0x7fffff00LL && recent >= 0 && recent <= keep, PQ_ERR_ARG,

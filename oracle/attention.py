@@ -65,7 +65,7 @@ def encode(x, scale):
     inv = np.float32(1) / scale if scale > 0 else np.float32(0)
     with np.errstate(over="ignore", invalid="ignore"):
         y = np.clip(np.rint(x * inv), -127, 127)
-    return np.where(np.isnan(x), 0, y).astype(np.int8)
+    return np.where(np.isnan(y), 0, y).astype(np.int8)   # NaN, and infinities of a page without a scale
 
 
 class Cache:

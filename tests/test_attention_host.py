@@ -1,0 +1,196 @@
+"""Host side of the attention ops on the CPU: schemas, fake kernels, refusals of the Python layer and of the C entry
+points (all before any launch), workspace sizes."""
+
+import ctypes
+
+import pytest
+import torch
+
+import alpamayo_amd  # noqa: F401
+from alpamayo_amd import _lib, attention
+
+BF = torch.bfloat16
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _case(batch=2, heads=2, hq=4, d=64, tokens=3, pages=5, width=3):
+    return dict(q=torch.zeros(tokens, hq, d, dtype=BF), k=torch.zeros(tokens, heads, d, dtype=BF),
+                v=torch.zeros(tokens, heads, d, dtype=BF), k_cache=torch.zeros(pages, heads, 64, d, dtype=torch.int8),
+                v_cache=torch.zeros(pages, heads, d, 64, dtype=torch.int8), k_scale=torch.zeros(pages, heads),
+                v_scale=torch.zeros(pages, heads), table=torch.zeros(batch, width, dtype=torch.int32), cu=_i32([0, 1, 3]),
+                lens=_i32([1, 2]), lse=torch.zeros(hq, tokens), weights=torch.zeros(batch, heads, 10))
+
+
+CALLS = {
+    "prompt": (attention._prompt_impl, ("q", "k", "v", "cu")),
+    "append": (attention._append_impl, ("k", "v", "k_cache", "v_cache", "k_scale", "v_scale", "table", "cu", "lens")),
+    "cache": (attention._cache_attn_impl, ("q", "k_cache", "v_cache", "k_scale", "v_scale", "table", "cu", "lens")),
+    "weights": (attention._cache_weights_impl, ("q", "k_cache", "k_scale", "table", "cu", "lens", "lse", "weights")),
+    "evict": (attention._evict_impl, ("k_cache", "v_cache", "k_scale", "v_scale", "weights", "table", "lens", "table")),
+}
+
+
+def _call(name, case, *more):
+    fn, args = CALLS[name]
+    return fn(*(case[a] for a in args), *more)
+
+
+@pytest.mark.parametrize("name,change,text", [
+    ("prompt", dict(q=torch.zeros(3, 4, 64)), "q must be one of"),
+    ("prompt", dict(k=torch.zeros(3, 2, 64, dtype=torch.float16)), "k must be one of"),
+    ("prompt", dict(q=torch.zeros(3, 4, 32, dtype=BF)), "64 or 128"),
+    ("prompt", dict(q=torch.zeros(3, 5, 64, dtype=BF)), "not a multiple"),
+    ("prompt", dict(q=torch.zeros(3, 4, 128, dtype=BF)), "channels a head"),
+    ("prompt", dict(v=torch.zeros(3, 4, 64, dtype=BF)), "one shape"),
+    ("prompt", dict(q=torch.zeros(2, 4, 64, dtype=BF)), "give cu_seqlens_k"),
+    ("prompt", dict(cu=torch.tensor([0, 1, 3])), "int32"),
+    ("prompt", dict(cu=_i32([])), "batch \\+ 1"),
+    ("prompt", dict(cu=_i32([[0, 3]])), "must be"),
+    ("append", dict(k=torch.zeros(3, 2, 64, dtype=torch.int8)), "k must be one of"),
+    ("append", dict(k=torch.zeros(3, 4, 64, dtype=BF), v=torch.zeros(3, 4, 64, dtype=BF)), "as the cache"),
+    ("append", dict(k_cache=torch.zeros(5, 2, 32, 64, dtype=torch.int8)), "k_cache must be"),
+    ("append", dict(v_cache=torch.zeros(5, 2, 64, 128, dtype=torch.int8)), "v_cache must be"),
+    ("append", dict(k_scale=torch.zeros(5, 2, dtype=torch.float16)), "k_scale must be"),
+    ("append", dict(v_scale=torch.zeros(5, 4)[:, ::2]), "v_scale must be contiguous"),
+    ("append", dict(table=torch.zeros(3, 3, dtype=torch.int32)), "block_table must be"),
+    ("append", dict(lens=_i32([1])), "cached_lens must be"),
+    ("cache", dict(q=torch.zeros(3, 3, 64, dtype=BF)), "not a multiple"),
+    ("cache", dict(q=torch.zeros(3, 4, 128, dtype=BF)), "channels a head"),
+    ("cache", dict(lens=_i32([1, 2, 3])), "lens must be"),
+    ("cache", dict(table=torch.zeros(2, dtype=torch.int32)), "block_table must be"),
+    ("weights", dict(q=torch.zeros(3, 3, 64, dtype=BF)), "not a multiple"),
+    ("weights", dict(q=torch.zeros(3, dtype=BF)), "q must be"),
+    ("evict", dict(lens=_i32([[1, 2]])), "lens must be"),
+    ("evict", dict(table=torch.zeros(1, 3, dtype=torch.int32)), "block_table must be"),
+    ("evict", dict(v_scale=torch.zeros(4, 2)), "v_scale must be"),
+])
+def test_refusals(name, change, text):
+    more = (4, 1) if name == "evict" else ()
+    with pytest.raises(RuntimeError, match=text):
+        _call(name, {**_case(), **change}, *more)
+
+
+def test_fake_kernels():
+    m = {n: t.to("meta") for n, t in _case().items()}
+    ops = torch.ops.paroquant_attn
+    out, lse = ops.prompt_attention(m["q"], m["k"], m["v"], m["cu"])
+    assert out.shape == (3, 4, 64) and out.dtype == BF and lse.shape == (4, 3) and lse.dtype == torch.float32
+    pools = [m[n] for n in ("k_cache", "v_cache", "k_scale", "v_scale")]
+    assert ops.kv_append_i8(m["k"], m["v"], *pools, m["table"], m["cu"], m["lens"]) is None
+    out, lse = ops.cache_attention_i8(m["q"], *pools, m["table"], m["cu"], m["lens"])
+    assert out.shape == (3, 4, 64) and lse.shape == (4, 3)
+    w, left, kept = ops.cache_evict_i8(*pools, m["weights"], m["table"], m["lens"], m["table"], 7, 2)
+    assert w.shape == (2, 2, 10) and left.shape == (2,) and kept.shape == (2, 2, 7) and kept.dtype == torch.int32
+
+
+def test_no_cpu_implementation():
+    c = _case()
+    with pytest.raises(NotImplementedError):
+        attention.prompt_attention(c["q"], c["k"], c["v"], c["cu"])
+
+
+def test_cache_object_checks():
+    for args in ((4, 2, 96), (4, 0, 64), (-1, 2, 64)):
+        with pytest.raises(RuntimeError):
+            attention.PagedKVCacheI8(*args, device="cpu")
+    assert attention.PagedKVCacheI8(0, 2, 64, device="cpu").k_cache.shape == (0, 2, 64, 64)
+
+
+# The C entry points.  Buffers are never read: every call is refused before a launch.
+P = 4096            # an address that is aligned and not null
+
+
+def _prompt_args(**change):
+    a = dict(q=P, k=P, v=P, dtype=_lib.PQ_BF16, qs=256, qh=64, ks=128, kh=64, vs=128, vh=64, cq=P, ck=P, out=P, lse=P, batch=2,
+             tq=10, tk=10, heads=2, group=2, d=64, scale=0.1, causal=1, ws=None, wsb=0, stream=None)
+    a.update(change)
+    return list(a.values())
+
+
+def _append_args(**change):
+    a = dict(k=P, v=P, dtype=_lib.PQ_BF16, ks=128, kh=64, vs=128, vh=64, kc=P, vc=P, ksc=P, vsc=P, table=P, cu=P, cached=P, batch=2,
+             width=3, tokens=10, heads=2, d=64, pages=5, stream=None)
+    a.update(change)
+    return list(a.values())
+
+
+def _cache_args(**change):
+    a = dict(q=P, dtype=_lib.PQ_BF16, qs=256, qh=64, kc=P, vc=P, ksc=P, vsc=P, table=P, cu=P, lens=P, out=P, lse=P, batch=2, width=3,
+             tokens=10, heads=2, group=2, d=64, pages=5, scale=0.1, ws=P, wsb=1 << 40, stream=None)
+    a.update(change)
+    return list(a.values())
+
+
+def _weights_args(**change):
+    a = dict(q=P, dtype=_lib.PQ_BF16, qs=256, qh=64, kc=P, ksc=P, table=P, cu=P, lens=P, lse=P, weights=P, batch=2, width=3, span=9,
+             tokens=10, heads=2, group=2, d=64, pages=5, scale=0.1, stream=None)
+    a.update(change)
+    return list(a.values())
+
+
+def _evict_args(**change):
+    a = dict(kc=P, vc=P, ksc=P, vsc=P, weights=P, table=P, lens=P, new=P, wo=P, lo=P, kept=P, batch=2, width=3, new_width=3, span=9,
+             heads=2, d=64, pages=5, keep=100, recent=5, stream=None)
+    a.update(change)
+    return list(a.values())
+
+
+COMMON = [dict(d=96), dict(heads=0), dict(batch=-1), dict(batch=1 << 40), dict(pages=-1), dict(width=-1), dict(width=1 << 30)]
+
+
+@pytest.mark.parametrize("name,make,bad", [
+    ("pq_attn_prompt", _prompt_args,
+     [dict(dtype=_lib.PQ_F32), dict(d=32), dict(heads=0), dict(group=0), dict(heads=70000), dict(batch=-1), dict(batch=1 << 30),
+      dict(tq=-1), dict(tk=-1), dict(tq=1 << 31), dict(tk=1 << 31), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")),
+      dict(scale=float("nan")), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(lse=None), dict(cq=None),
+      dict(ck=None), dict(q=P + 2), dict(k=P + 8), dict(v=P + 2), dict(out=P + 2), dict(qs=129), dict(kh=4), dict(vs=-8),
+      dict(ks=(1 << 24) + 8), dict(tk=9000)]),       # the last: keys are split, no workspace
+    ("pq_kv_append_i8", _append_args, COMMON + [
+        dict(dtype=9), dict(tokens=-1), dict(heads=70000), dict(k=None), dict(v=None), dict(kc=None), dict(vc=None), dict(ksc=None),
+        dict(vsc=None), dict(table=None), dict(cu=None), dict(cached=None), dict(k=P + 8), dict(vc=P + 4), dict(ks=4), dict(vh=12)]),
+    ("pq_attn_cache_i8", _cache_args, COMMON + [
+        dict(dtype=_lib.PQ_F32), dict(group=0), dict(tokens=-1), dict(tokens=1 << 31), dict(scale=0.0), dict(q=None), dict(q=P + 4),
+        dict(qs=4), dict(cu=None), dict(lens=None), dict(table=None), dict(kc=None), dict(vc=None), dict(ksc=None), dict(vsc=None),
+        dict(out=None), dict(lse=None), dict(out=P + 8), dict(ws=None), dict(wsb=16), dict(ws=P + 8)]),
+    ("pq_attn_cache_weights_i8", _weights_args, COMMON + [
+        dict(dtype=_lib.PQ_F32), dict(span=-1), dict(scale=0.0), dict(q=None), dict(qh=3), dict(kc=None), dict(ksc=None),
+        dict(table=None), dict(cu=None), dict(lens=None), dict(lse=None), dict(weights=None)]),
+    ("pq_kv_evict_i8", _evict_args, COMMON + [
+        dict(heads=70000), dict(keep=0), dict(keep=1 << 31), dict(recent=-1), dict(recent=101), dict(span=-1), dict(span=1 << 31),
+        dict(new_width=1, width=9), dict(new_width=-1), dict(lens=None), dict(lo=None), dict(kept=None), dict(weights=None),
+        dict(wo=None), dict(table=None), dict(new=None), dict(kc=None), dict(vc=None), dict(ksc=None), dict(vsc=None),
+        dict(kc=P + 8)]),
+])
+def test_c_entry_points_refuse(name, make, bad):
+    fn = getattr(_lib.load(), name)
+    for change in bad:
+        assert fn(*make(**change)) != 0, f"{name} took {change}"
+        with pytest.raises(Exception, match=name):
+            _lib.check(fn(*make(**change)), name)
+
+
+def test_c_entry_points_without_work():
+    lib = _lib.load()
+    assert lib.pq_attn_prompt(*_prompt_args(tq=0)) == 0
+    for change in (dict(batch=0), dict(tokens=0), dict(width=0), dict(pages=0)):
+        assert lib.pq_kv_append_i8(*_append_args(**change)) == 0
+        assert lib.pq_attn_cache_weights_i8(*_weights_args(**change)) == 0
+    assert lib.pq_attn_cache_i8(*_cache_args(tokens=0)) == 0
+    assert lib.pq_kv_evict_i8(*_evict_args(batch=0)) == 0
+
+
+def test_workspace_sizes():
+    lib = _lib.load()
+    size = lib.pq_attn_prompt_workspace_size
+    assert size(1, 8192, 8192, 8, 4, 128) == 0 and size(0, 10, 10, 8, 4, 128) == 0 and size(1, 10, 0, 8, 4, 128) == 0
+    need = size(1, 128, 8192, 8, 4, 128)
+    # whole parts of (results, maximum, sum) for each row
+    assert need > 0 and need % (128 * 32 * 130 * 4) == 0
+    assert 2 <= need // (128 * 32 * 130 * 4) <= 64
+    size = lib.pq_attn_cache_i8_workspace_size
+    assert size(0, 5, 4, 128) == 0 and size(4, 0, 4, 128) == 0
+    assert size(4, 16, 4, 128) < size(4, 64, 4, 128)        # units of 16 rows, and of 64
+    assert ctypes.sizeof(ctypes.c_float) * 130 * 16 * 2 <= size(4, 16, 4, 128)

@@ -304,6 +304,12 @@ def test_cache_attention_split_over_many_workgroups():
     _cache_case([2, 1], [9001, 3], 2, 1, 128, HF, seed=5)
 
 
+def test_cache_attention_more_parts_than_lanes():
+    """One key/value head and row tile whose pages make a share for each of hundreds of workgroups."""
+    _cache_case([1], [131072], 2, 1, 64, BF, seed=8)
+    _cache_case([17], [60000], 2, 1, 128, HF, seed=9)
+
+
 def test_cache_attention_pages_that_do_not_exist():
     table = torch.tensor([[1, -1, 3], [50, 2, 0]], dtype=torch.int32)
     _cache_case([2, 1], [190, 100], 4, 2, 128, BF, seed=6, table=table, pages=5)

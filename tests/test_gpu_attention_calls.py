@@ -1,0 +1,468 @@
+"""How the attention ops and the cache are called: custom-op behaviour, refusals, graphs, streams, empty and very large
+inputs, and a decoder layer's run of them together."""
+
+import numpy as np
+import pytest
+import torch
+
+import alpamayo_amd  # noqa: F401
+from alpamayo_amd import attention, workloads
+from alpamayo_amd.attention import PagedKVCacheI8
+from alpamayo_amd.quantization import SharedInputRotateLinears
+from oracle import attention as oatt
+from tests.test_gpu_attention import BF, HF, PAGE, _check, _cu, _cuda, _gen, _np, _pools, _rand, _same_cache, _score_error, _table
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _setup(seed=0, batch=3, width=4, heads=2, hq=4, d=64, new=1, lens=(130, 64, 5), dtype=BF):
+    """q, new k and v, pools, table, offsets and lengths on the device."""
+    g = _gen(seed)
+    pools = _cuda(*_pools(g, 2 * batch * width + 1, heads, d))
+    both = _table(g, batch, 2 * width, 2 * batch * width + 1).cuda()
+    n = batch * new
+    q, k, v = (_rand(g, n, h, d, dtype=dtype).cuda() for h in (hq, heads, heads))
+    return dict(q=q, k=k, v=v, pools=pools, table=both[:, :width].contiguous(), new_table=both[:, width:].contiguous(),
+                cu=_cu([new] * batch).cuda(), lens=_i32(list(lens)), cached=_i32([x - new for x in lens]),
+                weights=torch.rand(batch, heads, width * PAGE, generator=g).cuda())
+
+
+def test_opcheck():
+    s = _setup()
+    _, lse = attention.cache_attention_i8(s["q"], *s["pools"], s["table"], s["cu"], s["lens"])
+    cu = _i32([0, 2, 3])
+    ops = torch.ops.paroquant_attn
+    cases = {
+        "prompt_attention": (ops.prompt_attention, (s["q"], s["k"], s["v"], cu)),
+        "kv_append_i8": (ops.kv_append_i8, (s["k"], s["v"], *s["pools"], s["table"], s["cu"], s["cached"])),
+        "cache_attention_i8": (ops.cache_attention_i8, (s["q"], *s["pools"], s["table"], s["cu"], s["lens"])),
+        "cache_weights_i8": (ops.cache_weights_i8, (s["q"], s["pools"][0], s["pools"][2], s["table"], s["cu"], s["lens"], lse,
+                                                    s["weights"])),
+        "cache_evict_i8": (ops.cache_evict_i8, (*s["pools"], s["weights"], s["table"], s["lens"], s["new_table"], 100, 10)),
+    }
+    registered = {n.split("::")[1].split(".")[0] for n in torch._C._dispatch_get_all_op_names() if n.startswith("paroquant_attn::")}
+    assert registered == set(cases)
+    for name, (op, args) in cases.items():
+        print(f"opcheck {name}", flush=True)
+        torch.library.opcheck(op, args)
+
+
+def test_inputs_that_record_gradients_are_refused():
+    s = _setup()
+    cu = _i32([0, 2, 3])
+    for name in "qkv":
+        rows = {n: s[n].clone().requires_grad_(n == name) for n in "qkv"}
+        with pytest.raises(RuntimeError, match="no backward"):
+            attention.prompt_attention(rows["q"], rows["k"], rows["v"], cu)
+        with torch.no_grad():
+            attention.prompt_attention(rows["q"], rows["k"], rows["v"], cu)
+    q, k = s["q"].clone().requires_grad_(), s["k"].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        attention.kv_append_i8(k, s["v"], *s["pools"], s["table"], s["cu"], s["cached"])
+    with pytest.raises(RuntimeError, match="no backward"):
+        attention.cache_attention_i8(q, *s["pools"], s["table"], s["cu"], s["lens"])
+    lse = torch.zeros(4, 3, device="cuda")
+    with pytest.raises(RuntimeError, match="no backward"):
+        attention.cache_weights_i8(q, s["pools"][0], s["pools"][2], s["table"], s["cu"], s["lens"], lse, s["weights"])
+    with pytest.raises(RuntimeError, match="no backward"):
+        attention.cache_evict_i8(*s["pools"], s["weights"].clone().requires_grad_(), s["table"], s["lens"], s["new_table"], 9, 1)
+    assert not attention.prompt_attention(s["q"], s["k"], s["v"], cu)[0].requires_grad
+
+
+def test_empty_inputs():
+    s = _setup()
+    before = [p.clone() for p in s["pools"]]
+    none = s["q"][:0]
+    zero = _i32([0])
+    # no tokens; no sequences; sequences without tokens
+    for cu in (zero, _i32([0, 0, 0, 0])):
+        out, lse = attention.prompt_attention(none, s["k"][:0], s["v"][:0], cu)
+        assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
+    out, lse = attention.prompt_attention(s["q"], s["k"], s["v"], zero)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    out, lse = attention.prompt_attention(s["q"], s["k"][:0], s["v"][:0], _i32([0, 3]), _i32([0, 0]))
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    t0, l0 = s["table"][:0], s["lens"][:0]
+    attention.kv_append_i8(s["k"][:0], s["v"][:0], *s["pools"], s["table"], _i32([0, 0, 0, 0]), s["cached"])
+    attention.kv_append_i8(s["k"], s["v"], *s["pools"], t0, zero, l0)
+    attention.kv_append_i8(s["k"], s["v"], *s["pools"], s["table"][:, :0], s["cu"], s["cached"])
+    out, lse = attention.cache_attention_i8(s["q"], *s["pools"], t0, zero, l0)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    out, lse = attention.cache_attention_i8(s["q"], *s["pools"], s["table"][:, :0], s["cu"], s["lens"])
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    assert attention.cache_attention_i8(none, *s["pools"], s["table"], _i32([0, 0, 0, 0]), s["lens"])[0].shape == (0, 4, 64)
+    nopools = [p[:0] for p in s["pools"]]
+    out, lse = attention.cache_attention_i8(s["q"], *nopools, s["table"], s["cu"], s["lens"])
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    w = s["weights"].clone()
+    attention.cache_weights_i8(s["q"], nopools[0], nopools[2], s["table"], s["cu"], s["lens"], lse, w)
+    attention.cache_weights_i8(s["q"], s["pools"][0], s["pools"][2], s["table"], s["cu"], s["lens"], lse, w[:, :, :0].contiguous())
+    attention.cache_weights_i8(s["q"], s["pools"][0], s["pools"][2], s["table"], s["cu"], s["lens"], lse, w)   # lse = -inf: rows that saw nothing
+    assert torch.equal(w, s["weights"])
+    got = attention.cache_evict_i8(*s["pools"], s["weights"][:0], t0, l0, t0, 5, 1)
+    assert got[0].shape == (0, 2, 256) and got[1].shape == (0,) and got[2].shape == (0, 2, 5)
+    _, left, kept = attention.cache_evict_i8(*s["pools"], s["weights"], s["table"], _i32([0, -3, 0]), s["new_table"], 5, 1)
+    assert (left == 0).all() and (kept == -1).all()
+    _, left, kept = attention.cache_evict_i8(*s["pools"], s["weights"][:, :, :0], s["table"], s["lens"], s["new_table"], 5, 1)
+    assert (left == 0).all() and (kept == -1).all()
+    assert all(torch.equal(a, b) for a, b in zip(before, s["pools"]))
+
+
+def test_a_page_that_does_not_exist_gives_nothing_whatever_page_0_holds():
+    """Its tokens are read from page 0 in its place: a scale there that is not finite must not come through."""
+    for new, hq, lens in ((1, 4, (130, 64, 5)), (20, 4, (150, 64, 20))):
+        s = _setup(new=new, hq=hq, lens=lens, seed=3)
+        page0 = (s["table"] == 0).nonzero()
+        s["table"][tuple(page0[0]) if len(page0) else (0, 0)] = -1
+        s["table"][0, 1] = -1
+        good, z = attention.cache_attention_i8(s["q"], *s["pools"], s["table"], s["cu"], s["lens"])
+        for bad in (float("nan"), float("inf")):
+            s["pools"][2][0] = s["pools"][3][0] = bad
+            got = attention.cache_attention_i8(s["q"], *s["pools"], s["table"], s["cu"], s["lens"])
+            assert torch.equal(got[0], good) and torch.equal(got[1], z)
+            w = torch.zeros_like(s["weights"])
+            attention.cache_weights_i8(s["q"], s["pools"][0], s["pools"][2], s["table"], s["cu"], s["lens"], z, w)
+            assert w.isfinite().all()
+        assert good.isfinite().all()
+
+
+def test_infinities_alone_in_a_page():
+    """A page whose scale is 0 holds zeros, infinities of its tokens too."""
+    s = _setup()
+    ref = oatt.Cache(*(p.cpu().numpy() for p in s["pools"]))
+    k, v = torch.full_like(s["k"], float("inf")), torch.full_like(s["v"], -float("inf"))
+    cached = _i32([64, 128, 0])
+    attention.kv_append_i8(k, v, *s["pools"], s["table"], s["cu"], cached)
+    ref.append(_np(k), _np(v), _np(s["table"]), _np(s["cu"]), _np(cached))
+    _same_cache(s["pools"], ref)
+
+
+def test_strides_that_are_copied():
+    """Rows that the kernels' 16-byte loads cannot take as they lie: an odd start, an odd stride, channels apart."""
+    s = _setup(new=3, lens=(130, 64, 5), d=128)
+    def odd(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:]
+        flat.copy_(t.reshape(-1))
+        return flat.view(t.shape)
+    def wide(t):
+        x = torch.empty(t.size(0), t.size(1), t.size(2) + 3, dtype=t.dtype, device="cuda")[:, :, :t.size(2)]
+        return x.copy_(t)
+    def apart(t):
+        return t.permute(2, 0, 1).contiguous().permute(1, 2, 0)
+    want = attention.prompt_attention(s["q"], s["k"], s["v"], s["cu"])
+    cwant = attention.cache_attention_i8(s["q"], *s["pools"], s["table"], s["cu"], s["lens"])
+    awant = [p.clone() for p in s["pools"]]
+    attention.kv_append_i8(s["k"], s["v"], *awant, s["table"], s["cu"], s["cached"])
+    for f in (odd, wide, apart):
+        q, k, v = f(s["q"]), f(s["k"]), f(s["v"])
+        got = attention.prompt_attention(q, k, v, s["cu"])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        got = attention.cache_attention_i8(q, *s["pools"], s["table"], s["cu"], s["lens"])
+        assert torch.equal(got[0], cwant[0]) and torch.equal(got[1], cwant[1])
+        pools = [p.clone() for p in s["pools"]]
+        attention.kv_append_i8(k, v, *pools, s["table"], s["cu"], s["cached"])
+        assert all(torch.equal(a, b) for a, b in zip(pools, awant))
+    # one set of keys and values for all heads and tokens: strides of 0
+    k, v = s["k"][:1, :1].expand_as(s["k"]), s["v"][:1, :1].expand_as(s["v"])
+    got = attention.prompt_attention(s["q"], k, v, s["cu"])
+    full = attention.prompt_attention(s["q"], k.contiguous(), v.contiguous(), s["cu"])
+    assert torch.equal(got[0], full[0]) and torch.equal(got[1], full[1])
+    # tables and lengths that are views
+    t = torch.stack([s["table"], s["table"]], -1)[..., 0]
+    ln, cu = (torch.stack([x, x], -1)[..., 0] for x in (s["lens"], s["cu"]))
+    got = attention.cache_attention_i8(s["q"], *s["pools"], t, cu, ln)
+    assert torch.equal(got[0], cwant[0]) and torch.equal(got[1], cwant[1])
+
+
+def test_rows_past_32_bit_offsets():
+    """Rows 2^24 values apart (the widest that are read as they lie) and further: offsets past 2^31 values."""
+    n, d = 131, 64
+    g = _gen(1)
+    q, k, v = (_rand(g, n, 1, d).cuda() for _ in range(3))
+    cu = _i32([0, 3, n])
+    want = attention.prompt_attention(q, k, v, cu)
+    for step in (1 << 24, (1 << 24) + 8):
+        far = torch.empty(n * step, dtype=BF, device="cuda")
+        rows = [far.as_strided((n, 1, d), (step, d, 1), 64 * i) for i in range(3)]
+        for r, x in zip(rows, (q, k, v)):
+            r.copy_(x)
+        print(f"rows {step} values apart", flush=True)
+        got = attention.prompt_attention(*rows, cu)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        pools = [_cuda(*_pools(_gen(2), 6, 1, d)) for _ in range(2)]
+        table, cached = _i32([[0, 1], [2, 3]]), _i32([0, 0])
+        attention.kv_append_i8(rows[1], rows[2], *pools[0], table, cu, cached)
+        attention.kv_append_i8(k, v, *pools[1], table, cu, cached)
+        assert all(torch.equal(a, b) for a, b in zip(*pools))
+        del far, rows, got
+
+
+def test_pools_past_32_bit_offsets():
+    """The last pages of pools of more than 2^32 bytes against the same pages in small ones."""
+    pages, heads, d, small = 70000, 8, 128, 24
+    base = pages - small
+    big = [torch.zeros(pages, heads, PAGE, d, dtype=torch.int8, device="cuda"),
+           torch.zeros(pages, heads, d, PAGE, dtype=torch.int8, device="cuda"),
+           torch.zeros(pages, heads, device="cuda"), torch.zeros(pages, heads, device="cuda")]
+    assert big[0].numel() > 2 ** 32
+    little = _cuda(*_pools(_gen(5), small, heads, d))
+    for b, s in zip(big, little):
+        b[base:] = s
+    g = _gen(6)
+    q, k, v = (_rand(g, 40, h, d).cuda() for h in (16, heads, heads))
+    table, cu, lens, cached = _table(g, 2, 6, small).cuda(), _i32([0, 39, 40]), _i32([300, 150]), _i32([261, 149])
+    free = torch.tensor(sorted(set(range(small)) - set(table.flatten().tolist())), dtype=torch.int32, device="cuda")[:8].view(2, 4)
+    res = []
+    for pools, off in ((big, base), (little, 0)):
+        t, f = table + off, free + off
+        attention.kv_append_i8(k, v, *pools, t, cu, cached)
+        out, lse = attention.cache_attention_i8(q, *pools, t, cu, lens)
+        w = torch.zeros(2, heads, 384, device="cuda")
+        attention.cache_weights_i8(q, pools[0], pools[2], t, cu, lens, lse, w)
+        ew, left, kept = attention.cache_evict_i8(*pools, w, t, lens, f, 200, 30)
+        res.append([out, lse, w, ew, left, kept, *(p[off:off + small] for p in pools)])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+    assert all((p[:base] == 0).all() for p in big)
+
+
+def test_graph_serves_other_lengths():
+    """A decode step captured once; tokens, tables and lengths change in place between replays, with eager work between.
+    Rows behind the last sequence belong to no one, as in a padded batch."""
+    batch, width, heads, hq, d = 4, 5, 2, 8, 128
+    g = _gen(21)
+    make = lambda: _cuda(*_pools(_gen(22), 45, heads, d))   # noqa: E731
+    pools, eager = make(), make()
+    q, k, v = (torch.zeros(batch, h, d, dtype=BF, device="cuda") for h in (hq, heads, heads))
+    table = torch.zeros(batch, width, dtype=torch.int32, device="cuda")
+    cu, lens, cached = _i32([0, 1, 2, 3, 4]), _i32([1] * batch), _i32([0] * batch)
+    w = torch.zeros(batch, heads, width * PAGE, device="cuda")
+    new_table = _i32(np.arange(20, 20 + batch * 2).reshape(batch, 2).tolist())
+
+    def step(pools, w):
+        attention.kv_append_i8(k, v, *pools, table, cu, cached)
+        out, lse = attention.cache_attention_i8(q, *pools, table, cu, lens)
+        attention.cache_weights_i8(q, pools[0], pools[2], table, cu, lens, lse, w)
+        return (out, lse) + attention.cache_evict_i8(*pools, w, table, lens, new_table, 100, 10)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(make(), torch.zeros_like(w))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step(pools, w)
+    for p, e in zip(pools, eager):
+        p.copy_(e)
+    w.zero_()
+    we = torch.zeros_like(w)
+    for i, (offsets, ln) in enumerate([([0, 1, 2, 3, 4], [1, 64, 65, 320]), ([0, 1, 1, 2, 2], [200, 0, 129, 7]),
+                                       ([0, 1, 2, 3, 4], [2, 65, 66, 300]), ([0, 0, 0, 0, 0], [9, 9, 9, 9]),
+                                       ([0, 1, 2, 3, 4], [131, 5, 64, 128])]):
+        for t in (q, k, v):
+            t.copy_(_rand(g, *t.shape))
+        table.copy_(torch.randperm(20, generator=g).view(batch, width))
+        cu.copy_(_i32(offsets))
+        lens.copy_(_i32(ln))
+        cached.copy_(torch.clamp(lens - (cu[1:] - cu[:-1]), min=0))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(eager, we)
+        print(f"replay {i}", flush=True)
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+        assert all(torch.equal(a, b) for a, b in zip(pools, eager)) and torch.equal(w, we)
+        assert (res[0][offsets[-1]:] == 0).all()
+
+
+def test_graph_of_prompts_with_split_keys():
+    """A captured prompt call whose keys are split, replayed on other lengths; a second graph beside it."""
+    g = _gen(23)
+    q, k, v = (torch.zeros(n, h, 64, dtype=HF, device="cuda") for n, h in ((48, 4), (3000, 2), (3000, 2)))
+    cq, ck = _i32([0, 48, 48]), _i32([0, 3000, 3000])
+    graphs, res = [], []
+    attention.prompt_attention(q, k, v, cq, ck)
+    torch.cuda.synchronize()
+    for causal in (True, False):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res.append(attention.prompt_attention(q, k, v, cq, ck, causal=causal))
+        graphs.append(graph)
+    for a, b in (([0, 48, 48], [0, 3000, 3000]), ([0, 20, 40], [0, 1000, 2200]), ([0, 0, 48], [0, 0, 64]), ([0, 1, 47], [0, 0, 2999])):
+        for t in (q, k, v):
+            t.copy_(_rand(g, *t.shape, dtype=HF))
+        cq.copy_(_i32(a))
+        ck.copy_(_i32(b))
+        for graph in graphs:
+            graph.replay()
+        for causal, (out, lse) in zip((True, False), res):
+            want = attention.prompt_attention(q, k, v, cq, ck, causal=causal)
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+def test_streams():
+    """Calls on two streams at once, on tensors made on the first: the same bits as one after the other."""
+    a, b = _setup(seed=31, lens=(250, 200, 5)), _setup(seed=32, lens=(7, 66, 256))
+    keys = [(_rand(_gen(33 + i), 2000, 2, 64).cuda(), _rand(_gen(35 + i), 2000, 2, 64).cuda()) for i in range(2)]
+    ck = _i32([0, 700, 1400, 2000])
+
+    def run(s, kv):
+        return (*attention.cache_attention_i8(s["q"], *s["pools"], s["table"], s["cu"], s["lens"]),
+                *attention.prompt_attention(s["q"], *kv, s["cu"], ck))
+
+    want = [run(s, kv) for s, kv in zip((a, b), keys)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run((a, b)[i], keys[i]))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for r in g:
+            assert all(torch.equal(x, y) for x, y in zip(r, w))
+
+
+def test_refusals():
+    s = _setup()
+    q, k, v, pools, table, cu, lens = (s[n] for n in ("q", "k", "v", "pools", "table", "cu", "lens"))
+    bad = [
+        lambda: attention.prompt_attention(q, k, v.half(), cu),
+        lambda: attention.prompt_attention(q.float(), k.float(), v.float(), cu),
+        lambda: attention.prompt_attention(q[:, :3], k, v, cu),
+        lambda: attention.prompt_attention(q[:, :, :32], k[:, :, :32], v[:, :, :32], cu),
+        lambda: attention.prompt_attention(q[0], k, v, cu),
+        lambda: attention.prompt_attention(q, k[:2], v, cu),
+        lambda: attention.prompt_attention(q[:2], k, v, cu),
+        lambda: attention.prompt_attention(q, k, v, cu.long()),
+        lambda: attention.prompt_attention(q, k, v, cu[:0]),
+        lambda: attention.prompt_attention(q, k, v, cu.cpu()),
+        lambda: attention.prompt_attention(q, k, v, cu, cu[:2]),
+        lambda: attention.prompt_attention(q, k, v, cu, scale=0.0),
+        lambda: attention.prompt_attention(q, k, v, cu, scale=float("nan")),
+        lambda: attention.prompt_attention(q, k, v, cu, scale=1e-60),
+        lambda: attention.kv_append_i8(k, v, pools[1], pools[0], *pools[2:], table, cu, s["cached"][:2]),
+        lambda: attention.kv_append_i8(k[:, :1], v[:, :1], *pools, table, cu, s["cached"]),
+        lambda: attention.kv_append_i8(k, v, pools[0].transpose(0, 1), *pools[1:], table, cu, s["cached"]),
+        lambda: attention.kv_append_i8(k, v, *pools[:3], pools[3].double(), table, cu, s["cached"]),
+        lambda: attention.kv_append_i8(k, v, *pools, table[:2], cu, s["cached"]),
+        lambda: attention.kv_append_i8(k.cpu(), v, *pools, table, cu, s["cached"]),
+        lambda: attention.cache_attention_i8(q, *pools, table, cu, lens[:2]),
+        lambda: attention.cache_attention_i8(q, *pools, table.float(), cu, lens),
+        lambda: attention.cache_attention_i8(q[:, :3], *pools, table, cu, lens),
+        lambda: attention.cache_attention_i8(q, pools[0][:, :, :32], *pools[1:], table, cu, lens),
+        lambda: attention.cache_weights_i8(q, pools[0], pools[2], table, cu, lens, torch.zeros(4, 2, device="cuda"), s["weights"]),
+        lambda: attention.cache_weights_i8(q, pools[0], pools[2], table, cu, lens, torch.zeros(4, 3, device="cuda"),
+                                           s["weights"].transpose(1, 2).contiguous().transpose(1, 2)),
+        lambda: attention.cache_weights_i8(q[0], pools[0], pools[2], table, cu, lens, torch.zeros(4, 3, device="cuda"), s["weights"]),
+        lambda: attention.cache_evict_i8(*pools, s["weights"], table, lens, s["new_table"], 0, 0),
+        lambda: attention.cache_evict_i8(*pools, s["weights"], table, lens, s["new_table"], 10, 11),
+        lambda: attention.cache_evict_i8(*pools, s["weights"], table, lens, s["new_table"], 10, -1),
+        lambda: attention.cache_evict_i8(*pools, s["weights"], table, lens, s["new_table"][:, :1].contiguous(), 100, 1),
+        lambda: attention.cache_evict_i8(*pools, s["weights"][:2], table, lens, s["new_table"], 10, 1),
+        lambda: attention.cache_evict_i8(*pools, s["weights"].double(), table, lens, s["new_table"], 10, 1),
+    ]
+    before = [p.clone() for p in pools]
+    for i, f in enumerate(bad):
+        print(f"refusal {i}", flush=True)
+        with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+            f()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, pools))
+
+
+def test_cache_object():
+    c = PagedKVCacheI8(7, 2, 64)
+    assert c.k_cache.shape == (7, 2, 64, 64) and c.v_cache.shape == (7, 2, 64, 64) and c.k_scale.shape == (7, 2)
+    assert [PagedKVCacheI8.pages_for(n) for n in (0, 1, 64, 65)] == [0, 1, 1, 2]
+    s = _setup(batch=1, width=3, lens=(130,), new=130)
+    table = _i32([[6, 0, 3]])
+    c.append(s["k"], s["v"], table, s["cu"], s["cached"])
+    out, lse = c.attention(s["q"], table, s["cu"], s["lens"], scale=0.2)
+    want = attention.cache_attention_i8(s["q"], *c.pools, table, s["cu"], s["lens"], 0.2)
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    w = torch.zeros(1, 2, 192, device="cuda")
+    c.add_weights(s["q"], table, s["cu"], s["lens"], lse, w, scale=0.2)
+    # every row's weights sum to 1, whatever its scores: 2 query heads and 130 tokens a key/value head
+    assert torch.allclose(w.sum(-1), torch.full((1, 2), 260.0, device="cuda"), rtol=1e-4)
+    _, left, kept = c.evict(w, table, s["lens"], _i32([[1, 2]]), 70, 10)
+    assert left.tolist() == [70] and torch.equal(kept[0, 0, -10:].cpu(), torch.arange(120, 130, dtype=torch.int32))
+
+
+def test_layer_with_its_cache():
+    """A decoder layer's attention as it is served: two prompts, a decode step and a verify block over the cache, the cache
+    cut to what was attended to, and another step.  q, k and v come from the layer's linears, out goes to its o linear;
+    every stage is checked against the oracle fed that stage's inputs."""
+    H, hq, hkv, d = 1024, 8, 2, 128
+    g = workloads.generator(77)
+    mods = [workloads.build_module(workloads.linear_spec(n, N, H, g), "cuda")
+            for n, N in (("q", hq * d), ("k", hkv * d), ("v", hkv * d), ("o", H))]
+    qkv = SharedInputRotateLinears(mods[:3])
+    cache = PagedKVCacheI8(16, hkv, d)
+    ref = oatt.Cache(*(p.cpu().numpy() for p in cache.pools))
+    table = _i32([[3, 1, 9, 4], [0, 7, 5, 2]])
+    tn, sc = _np(table), d ** -0.5
+    held = np.zeros(2, np.int32)
+
+    def project(n, seed):
+        x = workloads.activations(n, H, workloads.generator(seed)).cuda()
+        q, k, v = qkv(x)
+        return q.view(n, hq, d), k.view(n, hkv, d), v.view(n, hkv, d)
+
+    def out(o):
+        y = mods[3](o.reshape(-1, hq * d))
+        assert y.shape == (o.size(0), H) and y.isfinite().all()
+
+    with torch.no_grad():
+        lens = np.array([150, 77], np.int32)
+        cu = _cu(lens)
+        q, k, v = project(227, 1)
+        o, lse = attention.prompt_attention(q, k, v, cu.cuda())
+        _check(o, lse, oatt.packed_attention(_np(q), _np(k), _np(v), cu.numpy(), cu.numpy(), sc), BF, BF,
+               _score_error(_np(q), _np(k), sc), np.abs(_np(v)).max(), 150)
+        out(o)
+        cache.append(k, v, table, cu.cuda(), _i32(held.tolist()))
+        ref.append(_np(k), _np(v), tn, cu.numpy(), held)
+        _same_cache(cache.pools, ref)
+        held = lens
+        weights = torch.zeros(2, hkv, 256, device="cuda")
+        want_w = np.zeros(weights.shape)
+
+        def step(new, seed):
+            nonlocal held, want_w
+            cu = _cu(new)
+            q, k, v = project(sum(new), seed)
+            cache.append(k, v, table, cu.cuda(), _i32(held.tolist()))
+            ref.append(_np(k), _np(v), tn, cu.numpy(), held)
+            _same_cache(cache.pools, ref)
+            held = held + np.array(new, np.int32)
+            lens = _i32(held.tolist())
+            o, lse = cache.attention(q, table, cu.cuda(), lens)
+            delta = _score_error(_np(q), np.full((1, d), ref.ks.max() * 127), sc)
+            _check(o, lse, ref.attention(_np(q), tn, cu.numpy(), held, sc), BF, HF, delta, ref.vs.max() * 127, int(held.max()))
+            out(o)
+            cache.add_weights(q, table, cu.cuda(), lens, lse, weights)
+            add = ref.weights(_np(q), tn, cu.numpy(), held, _np(lse), sc, 256)
+            tol = (2 * delta + 2.0 ** -20 * (1 + np.abs(_np(lse)).max())) * add + 2.0 ** -20 * (want_w + add)
+            want_w = want_w + add
+            assert (np.abs(_np(weights) - want_w) <= tol + 1e-30).all()
+            want_w = _np(weights).astype(np.float64)
+
+        step([1, 1], 2)
+        step([16, 16], 3)
+        # to 100 tokens each, into pages of their own; the old ones are free again
+        new_table = _i32([[6, 8], [10, 11]])
+        w, left, kept = cache.evict(weights, table, _i32(held.tolist()), new_table, 100, 16)
+        rw, rl, rk = ref.evict(_np(weights), tn, held, _np(new_table), 100, 16)
+        assert np.array_equal(_np(w), rw) and np.array_equal(_np(left), rl) and np.array_equal(_np(kept), rk)
+        _same_cache(cache.pools, ref)
+        table = torch.cat([new_table, table[:, :2]], 1).contiguous()
+        tn, held, weights, want_w = _np(table), rl, w, rw.astype(np.float64)
+        step([1, 1], 4)
+        step([30, 1], 5)
