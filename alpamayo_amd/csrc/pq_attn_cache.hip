@@ -506,13 +506,12 @@ __global__ __launch_bounds__(kThreads, 2) void attn_cache_rows_kernel(CacheArgs 
   });
 }
 
-// Joins the partial results of the rows whose unit spans workgroups.  A workgroup takes four (query head, token) rows of a
-// token: a wave each, or, where the parts are many, its waves together on one row after the other.  Rows outside of the
-// sequences and rows of empty ones get zeros and lse = -inf.
+// Joins the partial results of the rows whose unit spans workgroups.  A wave for each (query head, token)
+// row: maxima and sums of up to 64 parts at a time, a lane each, then their results, kAhead of them in flight.  Rows
+// outside of the sequences and rows of empty ones get zeros and lse = -inf.
 template <int D, int kRows, bool BF16>
 __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) {
-  constexpr int kV = D / 64;
-  __shared__ float so[kWaves][D], sl[kWaves], sm[kWaves];
+  constexpr int kV = D / 64, kAhead = 16;
   using P = Plan<kRows>;
   const int token = blockIdx.x, t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -537,118 +536,71 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
     total += read_lane(incl, 63);
   }
   const int len = b < 0 ? 0 : seq_len(a, b);
-  const auto out_row = [&](int h) { return static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(token) * hq + h) * D; };
-  const auto lse_of = [&](int h) { return a.lse + static_cast<int64_t>(h) * a.tokens + token; };
+  const int h = blockIdx.y * kWaves + wave;
+  if (h >= hq) return;
+  uint16_t* const out = static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(token) * hq + h) * D + lane * kV;
+  float* const lse = a.lse + static_cast<int64_t>(h) * a.tokens + token;
   if (len == 0) {
-    const int h = blockIdx.y * kWaves + wave;
-    if (h < hq) {
 #pragma unroll
-      for (int k = 0; k < kV; ++k) out_row(h)[lane * kV + k] = 0;
-      if (lane == 0) *lse_of(h) = -INFINITY;
-    }
+    for (int k = 0; k < kV; ++k) out[k] = 0;
+    if (lane == 0) *lse = -INFINITY;
     return;
   }
   const Span sp = span_of(a.cu, b, a.tokens);
   const int npages = (len + kPage - 1) / kPage;
   const Shares shares(total, a.workers);
 
-  // parts w0 + first, w0 + first + step, ... of a row into m, l, o
-  struct Parts { int64_t begin, w0, w1; int r; };
-  const auto parts_of = [&](int h) {
-    const int head = h / a.group, row = (token - sp.first) * a.group + h - head * a.group;
-    Parts q;
-    q.begin = before + (static_cast<int64_t>(row / kRows) * a.heads + head) * P::size(npages);
-    q.w0 = shares.owner(q.begin + kLead);
-    q.w1 = shares.owner(q.begin + kLead + npages - 1);
-    q.r = row % kRows;
-    return q;
-  };
-  const auto gather = [&](const Parts& q, int first, int step, float& m, float& l, float (&o)[kV]) {
-    m = -INFINITY;
-    l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kV; ++k) o[k] = 0.0f;
-    constexpr int kAhead = 4;
-    for (int64_t w = q.w0 + first; w <= q.w1; w += kAhead * step) {
-      float pm[kAhead], pl[kAhead], po[kAhead][kV];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        pm[i] = -INFINITY;
-        pl[i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kV; ++k) po[i][k] = 0.0f;
-        const int64_t x = w + i * step;
-        if (x <= q.w1) {
-          const bool own = shares.begin(x) >= q.begin;   // the unit is the first of its share
-          const float* p = a.part + (2 * x + (own ? 0 : 1)) * part_floats<kRows, D>();
-          pm[i] = p[kRows * D + q.r];
-          pl[i] = p[kRows * D + kRows + q.r];
-#pragma unroll
-          for (int k = 0; k < kV; ++k) po[i][k] = p[q.r * D + lane * kV + k];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const float big = fmaxf(m, pm[i]), base = big == -INFINITY ? 0.0f : big;
-        const float ca = exp2_fast(m - base), cb = exp2_fast(pm[i] - base);
-        l = l * ca + pl[i] * cb;
-#pragma unroll
-        for (int k = 0; k < kV; ++k) o[k] = o[k] * ca + po[i][k] * cb;
-        m = big;
-      }
-    }
-  };
-  const auto write = [&](int h, float m, float l, const float (&o)[kV]) {
-    const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
-#pragma unroll
-    for (int k = 0; k < kV; ++k)
-      out_row(h)[lane * kV + k] = BF16 ? pq_f32_to_bf16(o[k] * inv) : pq_f32_to_f16(o[k] * inv);
-    if (lane == 0) *lse_of(h) = (m + log2_fast(l)) * kLn2;
-  };
+  const int head = h / a.group, row = (token - sp.first) * a.group + h - head * a.group, r = row % kRows;
+  const int64_t begin = before + (static_cast<int64_t>(row / kRows) * a.heads + head) * P::size(npages);
+  const int64_t w0 = shares.owner(begin + kLead), w1 = shares.owner(begin + kLead + npages - 1);
+  if (w0 == w1) return;   // written by the workgroup that had all of it
+  // the unit is the first of its share but for share w0, where another may be
+  const bool second = shares.begin(w0) < begin;
+  const auto part = [&](int64_t w) { return a.part + (2 * w + (second && w == w0 ? 1 : 0)) * part_floats<kRows, D>(); };
 
-  // heads of a unit's rows share their parts but not their first one: whether they are many is the same for all of them
-  if (npages <= 16 * shares.each) {
-    const int h = blockIdx.y * kWaves + wave;
-    if (h >= hq) return;
-    const Parts q = parts_of(h);
-    if (q.w0 == q.w1) return;   // written by the workgroup that had all of it
-    float m, l, o[kV];
-    gather(q, 0, 1, m, l, o);
-    write(h, m, l, o);
-    return;
-  }
-  for (int i = 0; i < kWaves; ++i) {
-    const int h = blockIdx.y * kWaves + i;
-    if (h >= hq) return;
-    const Parts q = parts_of(h);
-    float m, l, o[kV];
-    gather(q, wave, kWaves, m, l, o);
-    if (lane == 0) {
-      sm[wave] = m;
-      sl[wave] = l;
+  float m = -INFINITY, l = 0.0f, o[kV];
+#pragma unroll
+  for (int k = 0; k < kV; ++k) o[k] = 0.0f;
+  for (int64_t w = w0; w <= w1; w += 64) {
+    const int n = static_cast<int>(min(static_cast<int64_t>(64), w1 - w + 1));
+    float pm = -INFINITY, pl = 0.0f;
+    if (lane < n) {
+      const float* p = part(w + lane) + kRows * D + r;
+      pm = p[0];
+      pl = p[kRows];
     }
+    float big = pm;
 #pragma unroll
-    for (int k = 0; k < kV; ++k) so[wave][lane * kV + k] = o[k];
-    __syncthreads();
-    if (wave == 0) {
-      float big = sm[0];
+    for (int s = 32; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor(big, s));
+    big = fmaxf(big, m);
+    const float base = big == -INFINITY ? 0.0f : big, was = exp2_fast(m - base), f = exp2_fast(pm - base);
+    float sum = pl * f;
 #pragma unroll
-      for (int x = 1; x < kWaves; ++x) big = fmaxf(big, sm[x]);
-      const float base = big == -INFINITY ? 0.0f : big;
-      l = 0.0f;
+    for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+    l = l * was + sum;
 #pragma unroll
-      for (int k = 0; k < kV; ++k) o[k] = 0.0f;
+    for (int k = 0; k < kV; ++k) o[k] *= was;
+    m = big;
+    for (int i = 0; i < n; i += kAhead) {
+      float po[kAhead][kV];
 #pragma unroll
-      for (int x = 0; x < kWaves; ++x) {
-        const float f = exp2_fast(sm[x] - base);
-        l += sl[x] * f;
+      for (int j = 0; j < kAhead; ++j) {
+        const float* p = part(w + min(i + j, n - 1)) + r * D + lane * kV;
 #pragma unroll
-        for (int k = 0; k < kV; ++k) o[k] += so[x][lane * kV + k] * f;
+        for (int k = 0; k < kV; ++k) po[j][k] = p[k];
       }
-      write(h, big, l, o);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float c = i + j < n ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), min(i + j, 63))) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) o[k] = __builtin_fmaf(po[j][k], c, o[k]);
+      }
     }
-    __syncthreads();
   }
+  const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+#pragma unroll
+  for (int k = 0; k < kV; ++k) out[k] = BF16 ? pq_f32_to_bf16(o[k] * inv) : pq_f32_to_f16(o[k] * inv);
+  if (lane == 0) *lse = (m + log2_fast(l)) * kLn2;
 }
 
 // weights[b, head, j] += sum over the head's rows of exp(s_ij - lse_i).  A unit is all rows of a sequence and head, 64 of
