@@ -220,10 +220,10 @@ def _prompt_impl(q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale=None, causal=Tr
         heads, d, batch = k.size(1), k.size(2), cu_seqlens_q.numel() - 1
     sc = _scale(scale, d)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((qs[1], qs[0]), dtype=torch.float32, device=dev)
+    lse = q.new_empty((qs[1], qs[0]), dtype=torch.float32)
     lib = _lib.load()
     need = lib.pq_attn_prompt_workspace_size(batch, qs[0], ks[0], heads, qs[1] // heads, d)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     a, b, c = q.stride(), k.stride(), v.stride()
     _launch("paroquant_attn::prompt_attention", lib.pq_attn_prompt, dev, q.data_ptr(), k.data_ptr(),
             v.data_ptr(), _DT[dt], a[0], a[1], b[0], b[1], c[0], c[1], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
@@ -343,10 +343,10 @@ def _cache_attn_impl(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seql
     batch, group = cu_seqlens_q.numel() - 1, hq // heads
     sc = _scale(scale, d)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((hq, tokens), dtype=torch.float32, device=dev)
+    lse = q.new_empty((hq, tokens), dtype=torch.float32)
     lib = _lib.load()
     need = lib.pq_attn_cache_i8_workspace_size(batch, tokens, group, d)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = q.new_empty(need, dtype=torch.uint8)
     a = q.stride()
     _launch("paroquant_attn::cache_attention_i8", lib.pq_attn_cache_i8, dev, q.data_ptr(), _DT[q.dtype], a[0], a[1],
             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
@@ -452,7 +452,7 @@ def _evict_impl(k_cache, v_cache, k_scale, v_scale, weights, block_table, lens, 
     w = weights.contiguous()
     out = torch.empty_like(w)
     new_lens = torch.empty_like(lens)
-    kept = torch.empty((batch, heads, keep), dtype=torch.int32, device=dev)
+    kept = lens.new_empty((batch, heads, keep))
     _launch("paroquant_attn::cache_evict_i8", _lib.load().pq_kv_evict_i8, dev, k_cache.data_ptr(), v_cache.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), w.data_ptr(), block_table.data_ptr(), lens.data_ptr(),
             new_table.data_ptr(), out.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), batch, block_table.size(1),
