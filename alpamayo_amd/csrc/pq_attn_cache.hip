@@ -12,7 +12,7 @@
 // row of q is scaled by a power of two so that its largest value lies in
 // [2^14, 2^15): every bf16 or fp16 value within 2^28 of it is exact, and what
 // lies below counts for less than a float32 sum can hold.  p is rounded to
-// fp16 (half a step 2^-12 of values up to 1), sums and statistics are float32.
+// fp16 (half a step 2^-11 of the value), sums and statistics are float32.
 //
 // Both products are taken transposed: S^T = K Q^T with tokens as the rows of
 // the result, O^T = V^T P^T.  A lane then holds the scores of one row (column
@@ -26,6 +26,15 @@
 // workgroup take a segment's pages in turn and join at its end through LDS.
 // A unit that spans workgroups leaves partial results (at most two for each
 // workgroup), which the second kernel joins.
+//
+// What bounds it, at 32 query on 8 key/value heads of 128: a large decode
+// batch the cache's bytes (64 sequences, 505000 tokens, 1.03 GB: 181 us, 5.7
+// TB/s, where a kernel that only reads reaches 6.0-6.4); verify blocks of 16
+// tokens the vector instructions, 240 for a wave and page (8 sequences, 26000
+// tokens: 24 us, a quarter of it before the first page is there); one
+// sequence latency (1733 tokens: 7.4 us, join 3.9).  Shares for 256 or 384
+// workgroups, runs of shares for each XCD and non-temporal loads measured no
+// better.
 #include <algorithm>
 
 #include "pq_attn.h"
@@ -507,8 +516,9 @@ __global__ __launch_bounds__(kThreads, 2) void attn_cache_rows_kernel(CacheArgs 
 }
 
 // Joins the partial results of the rows whose unit spans workgroups.  A wave for each (query head, token)
-// row: maxima and sums of up to 64 parts at a time, a lane each, then their results, kAhead of them in flight.  Rows
-// outside of the sequences and rows of empty ones get zeros and lse = -inf.
+// row: maxima and sums of up to 64 parts at a time, a lane each, then their results, kAhead of them in flight (one sequence
+// of 20000 tokens, 64 parts a row, with 4 / 8 / 16 in flight: 10.9 / 9.0 / 8.4 us; 8 verify blocks 7.1 us).  Rows outside
+// of the sequences and rows of empty ones get zeros and lse = -inf.
 template <int D, int kRows, bool BF16>
 __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) {
   constexpr int kV = D / 64, kAhead = 16;
@@ -606,7 +616,8 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
 // weights[b, head, j] += sum over the head's rows of exp(s_ij - lse_i).  A unit is all rows of a sequence and head, 64 of
 // them at a time staged in LDS as operands; the waves take a segment's pages in turn, the next one's codes in flight.
 // Here tokens are the columns of the scores, so that the rows' sum is over a lane's own values and the four groups of
-// lanes, in an order of its own whatever the shares.
+// lanes, in an order of its own whatever the shares.  One row in 16 of the products is used at a decode step, and the bytes
+// bound it: 32 sequences, 129000 tokens, 140 MB in 31 us (4.5 TB/s); 16 tokens of one sequence of 4097 9 us, latency.
 template <int D, bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void attn_weights_kernel(CacheArgs a) {
   constexpr int kKs = D / 32, kChunk = 64;
@@ -701,7 +712,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_weights_kernel(CacheArgs a) 
   });
 }
 
-// Rows of a unit: 16 where the call's sequences have no more on the average, else 64.
+// Rows of a unit: 16 where the call's sequences have no more on the average, else 64.  8 sequences of 4000 keys in units of
+// 16 / 64 rows: with 16 rows 18.4 / 19.9 us, with 20 25.6 / 22.6, with 64 40.3 / 26.3; 8 of 20000 with 4 rows 57 / 67.
 int unit_rows(int64_t batch, int64_t tokens, int64_t group) { return tokens * group <= 16 * batch ? 16 : 64; }
 
 int check(const char* who, const void* q, int dtype, int64_t q_st, int64_t q_sh, const void* k_cache, const void* k_scale,

@@ -14,8 +14,19 @@
 // the second product's operand as they stand.  V^T comes from LDS through the
 // transposing reads.
 //
-// p is rounded to the inputs' type (half a step 2^-9 of the value in bf16,
-// 2^-12 in fp16, as the outputs are); scores, sums and statistics are float32.
+// p is rounded to the inputs' type (half a step 2^-8 of the value in bf16,
+// 2^-11 in fp16, as the outputs are); scores, sums and statistics are float32.
+//
+// What bounds it: the two products and the softmax between them take about
+// the same issue time (d = 128: 1024 cycles of matrix instructions for a wave
+// and tile, of its vector instructions 512 for the exponentials and about as
+// many for maxima, sums and packing), and the card lowers its clock where
+// both run at once.  8192 tokens of 32 query on 8 key/value heads of 128:
+// 519-585 us, 940-1060 TFLOP/s, where a library product of 8192^3 reaches
+// 1216; 2048 tokens 56 us; a call of three short prompts 9 us, which is its
+// way to the data and four tiles after one another.  Eight waves in two
+// groups that take turns with the matrix cores ran 528 against 540 us, at
+// twice the rows in a workgroup, which the smaller calls lack.
 #include <algorithm>
 #include <type_traits>
 
@@ -392,52 +403,59 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
     a.lse[(static_cast<int64_t>(head) * a.group + h) * a.tokens_q + sq.first + token] = (m + log2_fast(l)) * kLn2;
 }
 
-// Joins the parts of a row, a wave for each.
+// Joins the parts of a row, D / 4 lanes for each, kAhead parts in flight.
 template <int D, bool BF16>
 __global__ __launch_bounds__(kThreads) void attn_prompt_join_kernel(PromptArgs a) {
-  constexpr int kV = D / 64;
-  const int lane = lane_id(), hq = a.heads * a.group;
+  constexpr int kLanes = D / 4, kAhead = 4;
+  const int t = threadIdx.x, hq = a.heads * a.group, c = t % kLanes * 4;
   const int64_t all = static_cast<int64_t>(a.tokens_q) * hq;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + t / kLanes;
   const int token = static_cast<int>(row / hq), h = static_cast<int>(row % hq);
   // rows outside of the sequences are done
   if (row >= all || a.batch == 0 || token < scalar_load(a.cu_q) || token >= scalar_load(a.cu_q + a.batch)) return;
   const float* const stats = a.part + a.parts * all * D;
-  float pm = -INFINITY, pl = 0.0f;      // of part `lane`
-  if (lane < a.parts) {
-    pm = stats[lane * all + row];
-    pl = stats[(a.parts + lane) * all + row];
-  }
-  float m = pm;
+  float m = -INFINITY, l = 0.0f;
+  f4 o = {0, 0, 0, 0};
+  for (int p0 = 0; p0 < a.parts; p0 += kAhead) {
+    float pm[kAhead], pl[kAhead];
+    f4 po[kAhead];
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-  const float f = m == -INFINITY ? 0.0f : exp2_fast(pm - m);
-  float l = pl * f, o[kV];
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t at = min(p0 + i, a.parts - 1) * all + row;
+      pm[i] = stats[at];
+      pl[i] = stats[a.parts * all + at];
+      po[i] = *reinterpret_cast<const f4*>(a.part + at * D + c);
+    }
+    float big = m;
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) l += __shfl_xor(l, s);
+    for (int i = 0; i < kAhead; ++i) big = fmaxf(big, pm[i]);
+    const float base = big == -INFINITY ? 0.0f : big, was = exp2_fast(m - base);
+    l *= was;
+    o *= was;
 #pragma unroll
-  for (int k = 0; k < kV; ++k) o[k] = 0.0f;
-  for (int p = 0; p < a.parts; ++p) {
-    const float c = __shfl(f, p);
-    if (c == 0.0f) continue;            // nothing, or nothing that counts
+    for (int i = 0; i < kAhead; ++i) {
+      const float f = p0 + i < a.parts ? exp2_fast(pm[i] - base) : 0.0f;
+      l = __builtin_fmaf(pl[i], f, l);
 #pragma unroll
-    for (int k = 0; k < kV; ++k) o[k] += a.part[(p * all + row) * D + lane * kV + k] * c;
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(f == 0.0f ? 0.0f : po[i][e], f, o[e]);   // 0: it may have left none
+    }
+    m = big;
   }
   const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
-#pragma unroll
-  for (int k = 0; k < kV; ++k) {
-    const float y = o[k] * inv;
-    a.out[row * D + lane * kV + k] = BF16 ? pq_f32_to_bf16(y) : pq_f32_to_f16(y);
-  }
-  if (lane == 0) a.lse[static_cast<int64_t>(h) * a.tokens_q + token] = (m + log2_fast(l)) * kLn2;
+  *reinterpret_cast<uint2*>(a.out + row * D + c) = make_uint2(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv));
+  if (c == 0) a.lse[static_cast<int64_t>(h) * a.tokens_q + token] = (m + log2_fast(l)) * kLn2;
 }
 
-// Parts of the keys for a call: as many as find room on the card (two workgroups a CU), of four key tiles or more on the
-// average (512 queries on 4101 keys 81 -> TBD us, 1024 on 1024 28 us either way).
+// Parts of the keys for a call: as many as find room on the card (two workgroups a CU), with `least` key tiles or more on
+// the average of a causal call.  With 32 query on 8 key/value heads of 128, whole / in parts: 1 query on 5000 keys 82 / 14
+// us, 128 on 8192 145 / 36, 512 on 4101 83 / 52, 1024 on 8192 170 / 147.  Two rounds of workgroups in parts lose: 512 on
+// 4101 52 / 67.  least: 64 queries on 1024 keys 25 us whole, 21 at 6, 18 at 3; 1024 on 1024, where the workgroups are 256,
+// 28 us whole and 36 at 4; 1024 on 1024 with 16 heads of 64 17.5 whole and 19.7 at 4.
 int parts_of(int64_t batch, int64_t tokens_q, int64_t tokens_k, int64_t kv_heads, int64_t group) {
-  const int64_t wgs = (tokens_q * group / kRows + std::min(batch, tokens_q)) * kv_heads;
-  const int64_t room = 512 / std::max<int64_t>(wgs, 1), tiles = tokens_k / kKeys / std::max<int64_t>(batch, 1);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({room, tiles / 4, 64})));
+  const int64_t wgs = batch * ((tokens_q / batch * group + kRows - 1) / kRows) * kv_heads;
+  const int64_t room = 512 / std::max<int64_t>(wgs, 1), tiles = (tokens_k - std::min(tokens_q, tokens_k) / 2) / batch / kKeys;
+  const int64_t least = wgs <= 64 ? 3 : 6;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({room, tiles / least, 64})));
 }
 
 }  // namespace
@@ -496,7 +514,8 @@ extern "C" int pq_attn_prompt(const void* q, const void* k, const void* v, int d
   PQ_REQUIRE(tiles * kv_heads * a.parts <= 0x7fffffffLL, PQ_ERR_ARG, "%s: too many rows", who);
   a.tiles = static_cast<int>(tiles);
   const unsigned grid = static_cast<unsigned>(tiles * kv_heads * a.parts);
-  const unsigned join = static_cast<unsigned>((tokens_q * kv_heads * group + kWaves - 1) / kWaves);
+  const int64_t each = kThreads / (head_dim / 4);   // rows of a workgroup that joins
+  const unsigned join = static_cast<unsigned>((tokens_q * kv_heads * group + each - 1) / each);
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define PQ_PROMPT(D_, BF_)                                                                       \
   do {                                                                                           \

@@ -12,7 +12,12 @@
 // finite values only, so one bad value does not wipe out its page: infinities
 // saturate, NaN is held as 0.
 //
-// One workgroup per touched page and head; no two write the same.  Every byte of a page outside of what is written stays as it was.
+// One workgroup per touched page and head; no two write the same.  Every byte
+// of a page outside of what is written stays as it was.
+//
+// What bounds it: long prompts their bytes (32293 tokens of 8 heads of 128,
+// 199 MB: 41 us, 4.8 TB/s, a copy's rate), a decode step the way to the data,
+// five reads after one another (7.4 us).
 #include "pq_attn.h"
 
 namespace {

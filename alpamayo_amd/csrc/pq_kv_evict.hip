@@ -9,6 +9,11 @@
 // the tokens once and writes the kept positions in order.  The second moves: one
 // workgroup per new page and head gathers its 64 tokens and rounds them to the
 // new page's scales, absmax / 127 of the values that they stand for.
+//
+// What bounds it: the pick its barriers and the atomics of a workgroup (4097
+// tokens 14 us, 32 sequences of 1500-13931 26 us), the move its reads: the V
+// rows of every page that something is kept of are read whole, 780 MB for 32
+// sequences cut to 4096 tokens (150 us, 5.2 TB/s).
 #include "pq_attn.h"
 
 namespace {
