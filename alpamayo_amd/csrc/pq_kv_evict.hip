@@ -11,9 +11,11 @@
 // new page's scales, absmax / 127 of the values that they stand for.
 //
 // What bounds it: the pick its barriers and the atomics of a workgroup (4097
-// tokens 14 us, 32 sequences of 1500-13931 26 us), the move its reads: the V
+// tokens 11 us, 32 sequences of 1500-13931 26 us), the move its reads: the V
 // rows of every page that something is kept of are read whole, 780 MB for 32
 // sequences cut to 4096 tokens (150 us, 5.2 TB/s).
+#include <algorithm>
+
 #include "pq_attn.h"
 
 namespace {
@@ -23,8 +25,6 @@ using namespace pqa;
 constexpr int kPickThreads = 1024;
 constexpr int kPickWaves = kPickThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kOwn = 16;                        // weights of a thread, in a block of
-constexpr int kBlock = kPickThreads * kOwn;
 constexpr int kMoveThreads = 256;
 
 // Unsigned keys in the order of the weights; NaN lowest, -0 as 0.
@@ -62,7 +62,10 @@ __device__ __forceinline__ uint32_t block_before(uint32_t x, uint32_t (&sums)[kP
   return before;
 }
 
+// kOwn: weights of a thread, kBlock of them held at once.
+template <int kOwn>
 __global__ __launch_bounds__(kPickThreads) void kv_pick_kernel(PickArgs a) {
+  constexpr int kBlock = kPickThreads * kOwn;
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t sums[kPickWaves];
   __shared__ uint32_t chosen, rest;
@@ -369,7 +372,14 @@ extern "C" int pq_kv_evict_i8(int8_t* k_cache, int8_t* v_cache, float* k_scale, 
   p.weights = weights; p.lens = lens; p.weights_out = weights_out; p.lens_out = lens_out; p.kept = kept;
   p.heads = static_cast<int>(heads); p.width = static_cast<int>(table_width);
   p.keep = static_cast<int>(keep); p.recent = static_cast<int>(recent); p.span = span;
-  kv_pick_kernel<<<dim3(static_cast<unsigned>(heads), static_cast<unsigned>(batch)), kPickThreads, 0, s>>>(p);
+  // The smallest block that holds a row's weights, which are then read once.  One sequence with blocks of 4 / 8 / 16
+  // thousand: 4000 weights 8.6 / 10.1 / 13.9 us, 8000 12.4 / 10.8 / 14.2, 16000 19.1 / 18.6 / 17.3 (32 thousand: 25.6),
+  // 60000 55 / 51 / 51 (59).
+  const dim3 pick(static_cast<unsigned>(heads), static_cast<unsigned>(batch));
+  const int64_t most = std::min(span, table_width * kPage);
+  if (most <= 4 * kPickThreads) kv_pick_kernel<4><<<pick, kPickThreads, 0, s>>>(p);
+  else if (most <= 8 * kPickThreads) kv_pick_kernel<8><<<pick, kPickThreads, 0, s>>>(p);
+  else kv_pick_kernel<16><<<pick, kPickThreads, 0, s>>>(p);
   if (pages > 0 && table_width > 0 && span > 0) {
     MoveArgs m;
     m.cache[0] = k_cache; m.cache[1] = v_cache; m.scale[0] = k_scale; m.scale[1] = v_scale;

@@ -373,6 +373,14 @@ def test_evict(lens, keep, recent, d):
     _evict_case(lens, keep, recent, 2, d, w, seed=d + keep)
 
 
+@pytest.mark.parametrize("n", [4096, 4097, 8192, 8200, 16384, 40001])
+def test_evict_long_rows(n):
+    """Rows of one and of several blocks of weights, with ties across their ends."""
+    w = torch.randint(0, 50, (1, 1, n), generator=_gen(n)).float()
+    _evict_case([n], n // 3, 100, 1, 64, w, seed=n)
+    _evict_case([n - 1], n - 2, 0, 1, 64, w[:, :, :n - 1].contiguous(), seed=n)
+
+
 def test_evict_ties_and_strange_weights():
     """Equal weights go to the earlier token; signed zeros are equal; NaN is lowest, infinities are the ends."""
     g = _gen(3)
