@@ -12,8 +12,9 @@
 //
 // What bounds it: the pick its barriers and the atomics of a workgroup (4097
 // tokens 11 us, 32 sequences of 1500-13931 26 us), the move its reads: the V
-// rows of every page that something is kept of are read whole, 780 MB for 32
-// sequences cut to 4096 tokens (150 us, 5.2 TB/s).
+// rows of every page that something is kept of are read whole, 780 MB with all
+// else for 32 sequences cut to 4096 tokens, of which 741 go past the L2 (136
+// us, 5.4 TB/s).
 #include <algorithm>
 
 #include "pq_attn.h"
@@ -235,9 +236,9 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(MoveArgs a) {
     kw[r] = *reinterpret_cast<const u4*>(a.cache[0] + src[k] + place[k] % kPage * D + c * 16);
   }
   const int tok = t & 63, d0 = t >> 6;
-  float v[kOwnCodes];
+  int vc[kOwnCodes];
 #pragma unroll
-  for (int r = 0; r < kOwnCodes; ++r) v[r] = 0.0f;
+  for (int r = 0; r < kOwnCodes; ++r) vc[r] = 0;
   const int mine = tok < count ? place[tok] / kPage : -1, slot = place[tok] % kPage;
   // tokens from `done` on are left; the pages of the next ones, in order and without repeats, up to kStaged
   for (int done = 0; done < count;) {
@@ -272,29 +273,43 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(MoveArgs a) {
         for (int q = 0; q < D / 64; ++q)
           *reinterpret_cast<u4*>(stage + i * (kPage * D) + (q * kMoveThreads + t) * 16) = w[i][q];
     __syncthreads();
+    int from_stage = -1;
 #pragma unroll
     for (int i = 0; i < kStaged; ++i)
-      if (mine >= 0 && mine == pages[i]) {
+      if (mine >= 0 && mine == pages[i]) from_stage = i;
+    if (from_stage >= 0) {
+      const int8_t* p = stage + from_stage * (kPage * D) + d0 * kPage + slot;
 #pragma unroll
-        for (int r = 0; r < kOwnCodes; ++r)
-          v[r] = static_cast<float>(stage[i * (kPage * D) + (d0 + 4 * r) * kPage + slot]) * mult[1][tok];
-      }
+      for (int r = 0; r < kOwnCodes; ++r) vc[r] = p[4 * r * kPage];
+    }
     __syncthreads();
     done = next;
   }
 
-  const auto magnitude = [](float x) {
-    const uint32_t m = __float_as_uint(x) & 0x7fffffffu;
-    return m < 0x7f800000u ? m : 0u;
-  };
   uint32_t big[2] = {0, 0};
-  float x[kOwnCodes];
+  float x[kOwnCodes], v[kOwnCodes];
+  float topk = 0.0f, topv = 0.0f;
 #pragma unroll
   for (int r = 0; r < kOwnCodes; ++r) {
     const int k = (t + r / 16 * kMoveThreads) / (D / 16);
     x[r] = static_cast<float>(static_cast<int8_t>(kw[r / 16][(r % 16) >> 2] >> (8 * (r & 3)))) * mult[0][k];
-    big[0] = max(big[0], magnitude(x[r]));
-    big[1] = max(big[1], magnitude(v[r]));
+    v[r] = static_cast<float>(vc[r]) * mult[1][tok];
+    topk = fmaxf(topk, fabsf(x[r]));
+    topv = fmaxf(topv, fabsf(v[r]));
+  }
+  big[0] = __float_as_uint(topk);
+  big[1] = __float_as_uint(topv);
+  if (__any(topk == INFINITY || topv == INFINITY)) {   // a page whose scale is not finite: the largest finite value
+    const auto magnitude = [](float y) {
+      const uint32_t m = __float_as_uint(y) & 0x7fffffffu;
+      return m < 0x7f800000u ? m : 0u;
+    };
+    big[0] = big[1] = 0;
+#pragma unroll
+    for (int r = 0; r < kOwnCodes; ++r) {
+      big[0] = max(big[0], magnitude(x[r]));
+      big[1] = max(big[1], magnitude(v[r]));
+    }
   }
   pq_wave_umax_n(big);
   if ((t & 63) == 0) {
@@ -322,16 +337,20 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(MoveArgs a) {
     *reinterpret_cast<u4*>(out + k * D + c * 16) = w;
   }
   out = a.cache[1] + ph * (kPage * D);
-  if (count == kPage) {
+  // the codes of token `tok`, channels d0, d0 + 4, ..., into a page
+  const auto put = [&](int8_t* to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < kOwnCodes; ++r) stage[(d0 + 4 * r) * kPage + tok] = static_cast<int8_t>(code_of(v[r], inv[1]));
+    for (int r = 0; r < kOwnCodes; ++r)
+      to[(d0 + 4 * r) * kPage + tok] = static_cast<int8_t>(code_of(v[r], inv[1]));
+  };
+  if (count == kPage) {
+    put(stage);
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < D / 64; ++q)
       *reinterpret_cast<u4*>(out + (q * kMoveThreads + t) * 16) = *reinterpret_cast<const u4*>(stage + (q * kMoveThreads + t) * 16);
   } else if (tok < count) {
-#pragma unroll
-    for (int r = 0; r < kOwnCodes; ++r) out[(d0 + 4 * r) * kPage + tok] = static_cast<int8_t>(code_of(v[r], inv[1]));
+    put(out);
   }
   if (t == 0) a.scale[0][ph] = now[0];
   if (t == 1) a.scale[1][ph] = now[1];

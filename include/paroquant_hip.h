@@ -489,7 +489,8 @@ int pq_attn_prompt(const void* q, const void* k, const void* v, int dtype, int64
  * codes become round(code * (old / new)); a page whose first token is new starts
  * afresh.  NaN counts as 0, infinities saturate and do not count for the
  * scale; a page whose absmax is below 2^-100 holds zeros.  Tokens whose page
- * does not exist are dropped.  No page may belong to two sequences of a call. */
+ * does not exist are dropped.  No page that a call writes to may belong to two
+ * of its sequences. */
 int pq_kv_append_i8(const void* k, const void* v, int dtype, int64_t k_stride_token, int64_t k_stride_head,
                     int64_t v_stride_token, int64_t v_stride_head, int8_t* k_cache, int8_t* v_cache, float* k_scale,
                     float* v_scale, const int32_t* block_table, const int32_t* cu_seqlens, const int32_t* cached_lens,
@@ -502,10 +503,10 @@ size_t pq_attn_cache_i8_workspace_size(int64_t batch, int64_t tokens, int64_t gr
 
 /* Attention of each sequence's last tokens over its cache.  q, out [tokens,
  * kv_heads * group, head_dim] and lse as for pq_attn_prompt; lens[b] (device
- * memory): tokens of sequence b in the cache, the new ones among them; query
- * i of n sees tokens j <= i + lens[b] - n.  workspace: 16-byte aligned; its
- * content does not matter, and calls that may run at the same time must not
- * share one. */
+ * memory): tokens of sequence b in the cache, the new ones among them (at most
+ * table_width * 64: more count as that); query i of n sees tokens j <= i +
+ * lens[b] - n.  workspace: 16-byte aligned; its content does not matter, and
+ * calls that may run at the same time must not share one. */
 int pq_attn_cache_i8(const void* q, int dtype, int64_t q_stride_token, int64_t q_stride_head, const int8_t* k_cache,
                      const int8_t* v_cache, const float* k_scale, const float* v_scale, const int32_t* block_table,
                      const int32_t* cu_seqlens, const int32_t* lens, void* out, float* lse, int64_t batch,

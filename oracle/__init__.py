@@ -23,6 +23,8 @@ the path so that the HIP kernels can be checked against it:
                of rotation::rotate_and_quant, rotation.cu:62-111)
   w4a16.py     the W4A16 linear: WQLinear.forward (qmodule.py:207-232) and
                RotateLinearInt4 over it (rotation_linear.py:136-139)
+  attention.py attention in float64, and the paged int8 cache's scales and
+               codes to the bit
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and the ``cpu_baseline`` leg of
 ``bench.py`` may import this package, and only as the checker: the product
@@ -47,6 +49,8 @@ Pinning status of each function (how each is checked, see tests/test_oracle_*.py
               when sz = -s*z is representable, and a brute-force loop for
               the GEMM.  The external kernels' accumulation order and
               rounding are parity unpinned (not in the reference tree).
+  attention   torch's scaled_dot_product_attention in float64; the cache by
+              its definition on small examples and by its values' attention.
   mxfp4       E2M1 grid against the format's bit-level definition, E8M0
               bytes against torch.float8_e8m0fnu, rounding against an
               exhaustive nearest-value search with explicit ties, round trip

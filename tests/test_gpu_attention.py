@@ -395,6 +395,25 @@ def test_evict_ties_and_strange_weights():
         _evict_case([1500, 1300], keep, 50, 2, 64, w, seed=keep)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_evict_pages_whose_scale_is_not_finite_or_zero_or_large(d):
+    """What such a page stands for: NaN is held as 0, infinities as the largest code, and the scale is that of the rest."""
+    g = _gen(d)
+    pools = _pools(g, 12, 2, d)
+    top = float(np.finfo(np.float32).max)
+    for i, bad in enumerate((float("nan"), float("inf"), 0.0, top / 127, 1e-42, -0.25)):
+        pools[2][i, i % 2] = pools[3][i, (i + 1) % 2] = bad
+    table, new = torch.arange(8, dtype=torch.int32)[None], torch.tensor([[8, 9, 10, 11]], dtype=torch.int32)
+    ln, w = torch.tensor([500], dtype=torch.int32), torch.rand(1, 2, 500, generator=g)
+    dev = _cuda(*pools)
+    got = attention.cache_evict_i8(*dev, *_cuda(w, table, ln, new), 230, 20)
+    ref = oatt.Cache(*(p.numpy() for p in pools))
+    with np.errstate(all="ignore"):
+        want = ref.evict(w.numpy(), table.numpy(), ln.numpy(), new.numpy(), 230, 20)
+    assert all(np.array_equal(_np(a), b) for a, b in zip(got, want))
+    _same_cache([p[8:] for p in dev], oatt.Cache(*(p[8:] for p in (ref.k, ref.v, ref.ks, ref.vs))))
+
+
 def test_evict_span_shorter_than_the_cache_and_missing_pages():
     g = _gen(6)
     _evict_case([300, 100], 120, 20, 2, 128, torch.rand(2, 2, 150, generator=g), seed=4)
