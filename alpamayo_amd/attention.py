@@ -302,7 +302,7 @@ def kv_append_i8(k, v, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqle
     A page's scale for a head is the absmax of what it holds / 127, a code round(x / scale).  Where new tokens are larger
     than what their page holds, its codes are rounded to the new scale; a page whose first token is new starts afresh.
     NaN is held as 0, infinities as the largest code.  The lengths are the caller's to advance.  A page that is
-    written to may belong to one sequence of the call only; pages in front of it may be shared."""
+    written to may be named once only in block_table; sequences may share the pages in front of it."""
     torch.ops.paroquant_attn.kv_append_i8.default(k, v, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens,
                                                   cached_lens)
 
@@ -473,8 +473,8 @@ def cache_evict_i8(k_cache, v_cache, k_scale, v_scale, weights, block_table, len
     """Cuts the cache of each sequence and head to `keep` tokens, its last `recent` ones and those before them with the
     largest weights (of equals the earlier ones; NaN counts as the lowest): (weights, lens, kept).
 
-    What is kept moves in order to the front of the pages that new_table names, which no sequence of the call may be
-    using; the old pages are the caller's to free.  Codes are rounded to the new pages' scales.  Returned: the kept
+    What is kept moves in order to the front of the pages that new_table names, each once and none in use by a
+    sequence of the call; the old pages are the caller's to free.  Codes are rounded to the new pages' scales.  Returned: the kept
     tokens' weights in their new places with zeros behind, as large as `weights`; the new lengths; and the kept tokens'
     old places, int32 [batch, heads, keep], -1 behind the last.  A sequence of `keep` tokens or fewer is moved whole.
     Tokens past the end of block_table or of `weights` do not count."""

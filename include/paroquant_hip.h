@@ -489,8 +489,8 @@ int pq_attn_prompt(const void* q, const void* k, const void* v, int dtype, int64
  * codes become round(code * (old / new)); a page whose first token is new starts
  * afresh.  NaN counts as 0, infinities saturate and do not count for the
  * scale; a page whose absmax is below 2^-100 holds zeros.  Tokens whose page
- * does not exist are dropped.  No page that a call writes to may belong to two
- * of its sequences. */
+ * does not exist are dropped.  A page that a call writes to may be named once
+ * only in block_table. */
 int pq_kv_append_i8(const void* k, const void* v, int dtype, int64_t k_stride_token, int64_t k_stride_head,
                     int64_t v_stride_token, int64_t v_stride_head, int8_t* k_cache, int8_t* v_cache, float* k_scale,
                     float* v_scale, const int32_t* block_table, const int32_t* cu_seqlens, const int32_t* cached_lens,
@@ -526,8 +526,8 @@ int pq_attn_cache_weights_i8(const void* q, int dtype, int64_t q_stride_token, i
 /* Each head of each sequence keeps its last `recent` tokens and, of those
  * before them, the ones with the largest weights [batch, heads, span], `keep`
  * in all (equal weights: the earlier token; NaN: lowest).  They move in order
- * to the front of the pages of new_table [batch, new_width], which no
- * sequence of the call may be using, rounded to those pages' scales.
+ * to the front of the pages of new_table [batch, new_width], named once each
+ * and in use by no sequence of the call, rounded to those pages' scales.
  * weights_out [batch, heads, span]: their weights, zeros behind; lens_out
  * [batch]: the new lengths; kept int32 [batch, heads, keep]: their old places,
  * -1 behind.  The output buffers must not overlap the inputs. */

@@ -130,6 +130,55 @@ def test_a_page_that_does_not_exist_gives_nothing_whatever_page_0_holds():
         assert good.isfinite().all()
 
 
+def test_offsets_and_lengths_past_their_tensors():
+    """Offsets and lengths that a tensor does not hold count as its ends."""
+    s = _setup(new=4, lens=(130, 64, 5))
+    good, far = _i32([0, 5, 5, 12]), _i32([-7, 5, 5, 10 ** 9])
+    a, b = (attention.prompt_attention(s["q"], s["k"], s["v"], cu) for cu in (good, far))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    lens, long = _i32([256, 0, 5]), _i32([2 ** 31 - 1, -9, 5])        # the table has 4 pages
+    a, b = (attention.cache_attention_i8(s["q"], *s["pools"], s["table"], cu, ln) for cu, ln in ((good, lens), (far, long)))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    ws = []
+    for cu, ln in ((good, lens), (far, long)):
+        w = s["weights"].clone()
+        attention.cache_weights_i8(s["q"], s["pools"][0], s["pools"][2], s["table"], cu, ln, a[1], w)
+        ws.append(w)
+    assert torch.equal(*ws)
+    ends = []
+    for cu, cached in ((good, _i32([254, 0, 60])), (far, _i32([254, -3, 60]))):
+        pools = [p.clone() for p in s["pools"]]
+        attention.kv_append_i8(s["k"], s["v"], *pools, s["table"], cu, cached)
+        ends.append(pools)
+    assert all(torch.equal(x, y) for x, y in zip(*ends))
+    pools = [p.clone() for p in s["pools"]]
+    attention.kv_append_i8(s["k"], s["v"], *pools, s["table"], good, _i32([2 ** 31 - 1, 256, 2 ** 31 - 60]))   # all behind the table
+    assert all(torch.equal(x, y) for x, y in zip(pools, s["pools"]))
+    ends = []
+    for ln in (lens, long):
+        pools = [p.clone() for p in s["pools"]]
+        ends.append([*attention.cache_evict_i8(*pools, s["weights"], s["table"], ln, s["new_table"], 100, 9), *pools])
+    assert all(torch.equal(x, y) for x, y in zip(*ends))
+
+
+def test_a_chunk_of_many_rows_over_the_cache():
+    """A prompt's second half over its own cache, beside the attention of its rows: the same within the codes' rounding."""
+    n, half, d = 1500, 800, 128
+    g = _gen(41)
+    q, k, v = (_rand(g, n, h, d).cuda() for h in (8, 2, 2))
+    c = PagedKVCacheI8(30, 2, d)
+    table = torch.randperm(30, generator=g)[:24].view(1, 24).to(torch.int32).cuda()
+    c.append(k[:half], v[:half], table, _i32([0, half]), _i32([0]))
+    c.append(k[half:], v[half:], table, _i32([0, n - half]), _i32([half]))
+    out, lse = c.attention(q[half:], table, _i32([0, n - half]), _i32([n]))
+    ref = oatt.Cache(*(p.cpu().numpy() for p in c.pools))
+    rows = torch.arange(half, n, 97)        # some rows, each as a query of its own
+    for i in rows.tolist():
+        r = ref.attention(_np(q[i:i + 1]), _np(table), np.array([0, 1]), np.array([i + 1]), d ** -0.5)
+        _check(out[i - half:i - half + 1], lse[:, i - half:i - half + 1], r, BF, HF,
+               _score_error(_np(q[i:i + 1]), np.full((1, d), ref.ks.max() * 127), d ** -0.5), ref.vs.max() * 127, n)
+
+
 def test_infinities_alone_in_a_page():
     """A page whose scale is 0 holds zeros, infinities of its tokens too."""
     s = _setup()
