@@ -32,7 +32,7 @@
 // TB/s, where a kernel that only reads reaches 6.0-6.4); verify blocks of 16
 // tokens the vector instructions, 240 for a wave and page (8 sequences, 26000
 // tokens: 24 us, a quarter of it before the first page is there); one
-// sequence latency (1733 tokens: 7.4 us, join 3.9).  Shares for 256 or 384
+// sequence latency (1733 tokens: 7.4 us, join 4.1).  Shares for 256 or 384
 // workgroups, runs of shares for each XCD and non-temporal loads measured no
 // better.
 #include <algorithm>
@@ -515,13 +515,14 @@ __global__ __launch_bounds__(kThreads, 2) void attn_cache_rows_kernel(CacheArgs 
   });
 }
 
-// Joins the partial results of the rows whose unit spans workgroups.  A wave for each (query head, token)
-// row: maxima and sums of up to 64 parts at a time, a lane each, then their results, kAhead of them in flight (one sequence
-// of 20000 tokens, 64 parts a row, with 4 / 8 / 16 in flight: 10.9 / 9.0 / 8.4 us; 8 verify blocks 7.1 us).  Rows outside
-// of the sequences and rows of empty ones get zeros and lse = -inf.
-template <int D, int kRows, bool BF16>
+// Joins the partial results of the rows whose unit spans workgroups.  kTeam waves for each (query head, token) row, a wave's
+// parts kTeam apart: maxima and sums of up to 64 of them at a time, a lane each, then their results, kAhead of them in
+// flight (one sequence of 20000 tokens, a wave a row, with 4 / 8 / 16 in flight 10.9 / 9.0 / 8.4 us).  Rows outside of the
+// sequences and rows of empty ones get zeros and lse = -inf.
+template <int D, int kRows, bool BF16, int kTeam>
 __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) {
   constexpr int kV = D / 64, kAhead = 16;
+  __shared__ float so[kTeam > 1 ? kTeam : 1][D], sm[kWaves], sl[kWaves];
   using P = Plan<kRows>;
   const int token = blockIdx.x, t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -546,7 +547,7 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
     total += read_lane(incl, 63);
   }
   const int len = b < 0 ? 0 : seq_len(a, b);
-  const int h = blockIdx.y * kWaves + wave;
+  const int h = kTeam > 1 ? blockIdx.y : blockIdx.y * kWaves + wave, first = kTeam > 1 ? wave : 0;
   if (h >= hq) return;
   uint16_t* const out = static_cast<uint16_t*>(a.out) + (static_cast<int64_t>(token) * hq + h) * D + lane * kV;
   float* const lse = a.lse + static_cast<int64_t>(h) * a.tokens + token;
@@ -571,11 +572,11 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
   float m = -INFINITY, l = 0.0f, o[kV];
 #pragma unroll
   for (int k = 0; k < kV; ++k) o[k] = 0.0f;
-  for (int64_t w = w0; w <= w1; w += 64) {
-    const int n = static_cast<int>(min(static_cast<int64_t>(64), w1 - w + 1));
+  for (int64_t w = w0 + first; w <= w1; w += 64 * kTeam) {
+    const int n = static_cast<int>(min(static_cast<int64_t>(64), (w1 - w) / kTeam + 1));
     float pm = -INFINITY, pl = 0.0f;
     if (lane < n) {
-      const float* p = part(w + lane) + kRows * D + r;
+      const float* p = part(w + lane * kTeam) + kRows * D + r;
       pm = p[0];
       pl = p[kRows];
     }
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
       float po[kAhead][kV];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const float* p = part(w + min(i + j, n - 1)) + r * D + lane * kV;
+        const float* p = part(w + min(i + j, n - 1) * kTeam) + r * D + lane * kV;
 #pragma unroll
         for (int k = 0; k < kV; ++k) po[j][k] = p[k];
       }
@@ -605,6 +606,28 @@ __global__ __launch_bounds__(kThreads) void attn_cache_join_kernel(CacheArgs a) 
 #pragma unroll
         for (int k = 0; k < kV; ++k) o[k] = __builtin_fmaf(po[j][k], c, o[k]);
       }
+    }
+  }
+  if constexpr (kTeam > 1) {
+    if (lane == 0) {
+      sm[wave] = m;
+      sl[wave] = l;
+    }
+#pragma unroll
+    for (int k = 0; k < kV; ++k) so[wave][lane * kV + k] = o[k];
+    __syncthreads();
+    if (wave > 0) return;
+    for (int x = 1; x < kTeam; ++x) m = fmaxf(m, sm[x]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kV; ++k) o[k] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kTeam; ++x) {
+      const float f = exp2_fast(sm[x] - base);
+      l = __builtin_fmaf(sl[x], f, l);
+#pragma unroll
+      for (int k = 0; k < kV; ++k) o[k] = __builtin_fmaf(so[x][lane * kV + k], f, o[k]);
     }
   }
   const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
@@ -716,6 +739,15 @@ __global__ __launch_bounds__(kThreads, 2) void attn_weights_kernel(CacheArgs a) 
 // 16 / 64 rows: with 16 rows 18.4 / 19.9 us, with 20 25.6 / 22.6, with 64 40.3 / 26.3; 8 of 20000 with 4 rows 57 / 67.
 int unit_rows(int64_t batch, int64_t tokens, int64_t group) { return tokens * group <= 16 * batch ? 16 : 64; }
 
+// Whether a workgroup joins one row: where units are few, and so the parts of each many, and rows are few too.  Join of one
+// sequence, a wave / a workgroup for a row: 32 rows of 64 parts (20000 tokens) 8.5 / 6.2 us, 8 rows of 390 (100000) 30.6 /
+// 11.6, 512 rows of 64 8.8 / 7.1; 1024 rows of 30 5.6 / 6.9, 512 rows of 4 4.9 / 5.8; 32 rows of a part or two 4.1 / 4.3.
+bool team_joins(int64_t batch, int64_t tokens, int64_t heads, int64_t group) {
+  const int64_t unit = unit_rows(batch, tokens, group);
+  const int64_t units = batch * ((tokens * group / batch + unit - 1) / unit) * heads;
+  return units <= 32 && tokens * heads * group <= 512;
+}
+
 int check(const char* who, const void* q, int dtype, int64_t q_st, int64_t q_sh, const void* k_cache, const void* k_scale,
           const void* table, const void* cu, const void* lens, int64_t batch, int64_t width, int64_t tokens,
           int64_t heads, int64_t group, int64_t d, int64_t pages, float scale) {
@@ -771,7 +803,9 @@ extern "C" int pq_attn_cache_i8(const void* q, int dtype, int64_t q_stride_token
   a.pages = static_cast<int>(pages); a.workers = kWorkers;
   a.scale_log2 = scale * kLog2e;
   const bool few = batch == 0 || unit_rows(batch, tokens, group) == 16;
-  const dim3 join(static_cast<unsigned>(tokens), static_cast<unsigned>((kv_heads * group + kWaves - 1) / kWaves));
+  const bool team = batch > 0 && team_joins(batch, tokens, kv_heads, group);
+  const dim3 join(static_cast<unsigned>(tokens),
+                  static_cast<unsigned>(team ? kv_heads * group : (kv_heads * group + kWaves - 1) / kWaves));
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define PQ_CACHE(D_, BF_)                                                          \
   do {                                                                             \
@@ -779,8 +813,10 @@ extern "C" int pq_attn_cache_i8(const void* q, int dtype, int64_t q_stride_token
       if (few) attn_cache_kernel<D_, BF_><<<kWorkers, kThreads, 0, s>>>(a);        \
       else attn_cache_rows_kernel<D_, BF_><<<kWorkers, kThreads, 0, s>>>(a);       \
     }                                                                              \
-    if (few) attn_cache_join_kernel<D_, 16, BF_><<<join, kThreads, 0, s>>>(a);     \
-    else attn_cache_join_kernel<D_, 64, BF_><<<join, kThreads, 0, s>>>(a);         \
+    if (few && team) attn_cache_join_kernel<D_, 16, BF_, kWaves><<<join, kThreads, 0, s>>>(a);  \
+    else if (few) attn_cache_join_kernel<D_, 16, BF_, 1><<<join, kThreads, 0, s>>>(a);          \
+    else if (team) attn_cache_join_kernel<D_, 64, BF_, kWaves><<<join, kThreads, 0, s>>>(a);    \
+    else attn_cache_join_kernel<D_, 64, BF_, 1><<<join, kThreads, 0, s>>>(a);                   \
   } while (0)
   if (head_dim == 64 && dtype == PQ_BF16) PQ_CACHE(64, true);
   else if (head_dim == 64) PQ_CACHE(64, false);
