@@ -23,7 +23,7 @@
 // many for maxima, sums and packing), and the card lowers its clock where
 // both run at once.  8192 tokens of 32 query on 8 key/value heads of 128:
 // 519-585 us, 940-1060 TFLOP/s, where a library product of 8192^3 reaches
-// 1216; 2048 tokens 56 us; a call of three short prompts 9 us, which is its
+// 1216; 2048 tokens 55 us; a call of three short prompts 8 us, which is its
 // way to the data and four tiles after one another.  Eight waves in two
 // groups that take turns with the matrix cores ran 528 against 540 us, at
 // twice the rows in a workgroup, which the smaller calls lack.
@@ -373,8 +373,8 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
   }
 
   l = sum_xor32(l);
-  if (!valid) return;
   if (a.parts > 1) {
+    if (!valid) return;
     // [part][token][head] rows of results, then of maxima, then of sums; a part without keys leaves no results
     const int64_t all = static_cast<int64_t>(a.tokens_q) * a.heads * a.group;
     const int64_t at = part * all + (static_cast<int64_t>(sq.first) + token) * a.heads * a.group + head * a.group + h;
@@ -392,15 +392,39 @@ __global__ __launch_bounds__(kThreads, 2) void attn_prompt_kernel(PromptArgs a) 
     return;
   }
   const float inv = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
-  uint16_t* op = a.out + ((static_cast<int64_t>(sq.first) + token) * a.heads * a.group + head * a.group + h) * D;
+  if (valid && half == 0)
+    a.lse[(static_cast<int64_t>(head) * a.group + h) * a.tokens_q + sq.first + token] = (m + log2_fast(l)) * kLn2;
+  if constexpr (D == 64) {
+    if (!valid) return;
+    uint16_t* op = a.out + ((static_cast<int64_t>(sq.first) + token) * a.heads * a.group + head * a.group + h) * D;
+#pragma unroll
+    for (int i = 0; i < kDt; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<uint2*>(op + 32 * i + 2 * e + 4 * half) =
+            make_uint2(pack2<BF16>(o[i][e] * inv, o[i][e + 1] * inv), pack2<BF16>(o[i][e + 2] * inv, o[i][e + 3] * inv));
+    return;
+  }
+  // Rows of 256 bytes go out whole, 16 bytes a lane, through the stage that the last tile did not use (the wave's own 32 rows
+  // of it): 32 sequences of 100 tokens 31.1 -> 28.6 us, one of 45 7.8 -> 7.1.  Rows of 128 gain nothing by it (16 heads,
+  // 16 sequences of 300 16.1 -> 16.5).
+  constexpr int kChunks = D / 8, kEach = 64 / kChunks;
+  uint16_t* const own = &lds[(end - begin + kKeys - 1) / kKeys & 1][0][0] + wave * 32 * D;
 #pragma unroll
   for (int i = 0; i < kDt; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      *reinterpret_cast<uint2*>(op + 32 * i + 2 * e + 4 * half) =
-          make_uint2(pack2<BF16>(o[i][e] * inv, o[i][e + 1] * inv), pack2<BF16>(o[i][e + 2] * inv, o[i][e + 3] * inv));
-  if (half == 0)
-    a.lse[(static_cast<int64_t>(head) * a.group + h) * a.tokens_q + sq.first + token] = (m + log2_fast(l)) * kLn2;
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<uint2*>(own + col * D + ((4 * i + e) ^ (col & (kChunks - 1))) * 8 + 4 * half) = make_uint2(
+          pack2<BF16>(o[i][4 * e] * inv, o[i][4 * e + 1] * inv), pack2<BF16>(o[i][4 * e + 2] * inv, o[i][4 * e + 3] * inv));
+#pragma unroll
+  for (int i = 0; i < 32 / kEach; ++i) {
+    const int r = i * kEach + lane / kChunks, c8 = lane % kChunks, to = __shfl(token, r);
+    const u4 x = *reinterpret_cast<const u4*>(own + r * D + (c8 ^ (r & (kChunks - 1))) * 8);
+    if (wrow + r < rows) {
+      const int64_t at = (static_cast<int64_t>(sq.first) + to) * a.heads * a.group + head * a.group + (wrow + r - to * a.group);
+      *reinterpret_cast<u4*>(a.out + at * D + c8 * 8) = x;
+    }
+  }
 }
 
 // Joins the parts of a row, D / 4 lanes for each, kAhead parts in flight.
