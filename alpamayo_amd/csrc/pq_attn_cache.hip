@@ -755,9 +755,9 @@ int check(const char* who, const void* q, int dtype, int64_t q_st, int64_t q_sh,
   PQ_REQUIRE(d == 64 || d == 128, PQ_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 64, 128)", who, (long long)d);
   PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffLL && width >= 0 && width <= 0x7fffffffLL / kPage, PQ_ERR_ARG,
              "%s: batch=%lld table_width=%lld", who, (long long)batch, (long long)width);
-  PQ_REQUIRE(heads >= 1 && group >= 1 && heads * group <= 65535, PQ_ERR_ARG, "%s: kv_heads=%lld group=%lld", who,
+  PQ_REQUIRE(heads >= 1 && group >= 1 && heads <= 65535 && group <= 65535 && heads * group <= 65535, PQ_ERR_ARG, "%s: kv_heads=%lld group=%lld", who,
              (long long)heads, (long long)group);
-  PQ_REQUIRE(tokens >= 0 && tokens * group <= 0x7fffffffLL - 64 && pages >= 0 && pages <= 0x7fffffffLL, PQ_ERR_ARG,
+  PQ_REQUIRE(tokens >= 0 && tokens <= 0x7fffffffLL && tokens * group <= 0x7fffffffLL - 64 && pages >= 0 && pages <= 0x7fffffffLL, PQ_ERR_ARG,
              "%s: tokens=%lld pages=%lld", who, (long long)tokens, (long long)pages);
   PQ_REQUIRE(scale > 0.0f && scale < INFINITY, PQ_ERR_ARG, "%s: scale=%g must be positive and finite", who, scale);
   if (tokens == 0) return PQ_OK;

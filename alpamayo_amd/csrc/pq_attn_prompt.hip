@@ -501,10 +501,10 @@ extern "C" int pq_attn_prompt(const void* q, const void* k, const void* v, int d
   PQ_REQUIRE(dtype == PQ_F16 || dtype == PQ_BF16, PQ_ERR_UNSUPPORTED, "%s: dtype code %d (Half or BFloat16)", who, dtype);
   PQ_REQUIRE(head_dim == 64 || head_dim == 128, PQ_ERR_UNSUPPORTED, "%s: head_dim=%lld (supported: 64, 128)", who,
              (long long)head_dim);
-  PQ_REQUIRE(kv_heads >= 1 && group >= 1 && kv_heads * group <= 65535, PQ_ERR_ARG, "%s: kv_heads=%lld group=%lld", who,
+  PQ_REQUIRE(kv_heads >= 1 && group >= 1 && kv_heads <= 65535 && group <= 65535 && kv_heads * group <= 65535, PQ_ERR_ARG, "%s: kv_heads=%lld group=%lld", who,
              (long long)kv_heads, (long long)group);
   PQ_REQUIRE(batch >= 0 && batch <= 0x7fffffLL && tokens_q >= 0 && tokens_k >= 0 && tokens_k <= 0x7fffffffLL - 64 &&
-                 tokens_q * group <= 0x7fffffffLL - 128, PQ_ERR_ARG,
+                 tokens_q <= 0x7fffffffLL && tokens_q * group <= 0x7fffffffLL - 128, PQ_ERR_ARG,
              "%s: batch=%lld tokens_q=%lld tokens_k=%lld", who, (long long)batch, (long long)tokens_q, (long long)tokens_k);
   PQ_REQUIRE(scale > 0.0f && scale < INFINITY, PQ_ERR_ARG, "%s: scale=%g must be positive and finite", who, scale);
   if (tokens_q == 0) return PQ_OK;

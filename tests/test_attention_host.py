@@ -194,3 +194,18 @@ def test_workspace_sizes():
     assert size(0, 5, 4, 128) == 0 and size(4, 0, 4, 128) == 0
     assert size(4, 16, 4, 128) < size(4, 64, 4, 128)        # units of 16 rows, and of 64
     assert ctypes.sizeof(ctypes.c_float) * 130 * 16 * 2 <= size(4, 16, 4, 128)
+
+
+@pytest.mark.parametrize("name,make,bad", [
+    ("pq_attn_prompt", _prompt_args, [dict(tq=1 << 62, group=4), dict(heads=1 << 40, group=1 << 24), dict(tk=1 << 62)]),
+    ("pq_attn_cache_i8", _cache_args, [dict(tokens=1 << 62, group=4), dict(heads=1 << 40, group=1 << 24)]),
+    ("pq_attn_cache_weights_i8", _weights_args, [dict(tokens=1 << 62, group=4), dict(heads=1 << 40, group=1 << 24), dict(span=1 << 62)]),
+    ("pq_kv_append_i8", _append_args, [dict(tokens=1 << 62), dict(batch=1 << 62), dict(heads=1 << 62)]),
+    ("pq_kv_evict_i8", _evict_args, [dict(keep=1 << 62), dict(batch=1 << 62), dict(new_width=1 << 62), dict(span=1 << 62)]),
+])
+def test_sizes_whose_products_overflow_are_refused(name, make, bad):
+    fn = getattr(_lib.load(), name)
+    for change in bad:
+        st = fn(*make(**change))
+        with pytest.raises(Exception, match="PQ_ERR_ARG"):
+            _lib.check(st, name)
