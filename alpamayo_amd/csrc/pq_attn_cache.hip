@@ -678,6 +678,10 @@ __global__ __launch_bounds__(kThreads, 2) void attn_weights_kernel(CacheArgs a) 
       int p = sg.p0 + wave;
       int id = 0, id_next = 0;
       float ks = 0.0f;
+      // The lane's token of the page before, its sum so far and what the rows add to it.  It is written when the next page's
+      // codes are there: what is waited for then was asked for a page ago.
+      int64_t at = a.span;
+      float was = 0.0f, mine = 0.0f;
       if (p < sg.p1) {
         id = scalar_load(table + p);
         if (p + kWaves < sg.p1) id_next = scalar_load(table + p + kWaves);
@@ -697,12 +701,19 @@ __global__ __launch_bounds__(kThreads, 2) void attn_weights_kernel(CacheArgs a) 
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int k = 0; k < kKs; ++k) kf[q][k] = codes_f16(kr[q][k >> 1][2 * (k & 1)], kr[q][k >> 1][2 * (k & 1) + 1]);
+        // made here, so that the next codes come into the registers of these ones
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int k = 0; k < kKs; ++k) asm volatile("" : "+v"(kf[q][k]));
+        __builtin_amdgcn_sched_barrier(0);
+        if (at < a.span) weights[at] = was + mine;
+        const int64_t j = static_cast<int64_t>(p) * kPage + lane;
+        was = weights[min(j, a.span - 1)];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < 4; ++q) load_k<D, false>(a.kc + ph * (kPage * D), q, kr[q]);
         __builtin_amdgcn_sched_barrier(0);
-        const int64_t j = static_cast<int64_t>(p) * kPage + lane;
-        float was = 0.0f;
-        if (j < a.span) was = weights[j];
         float sum[4] = {0, 0, 0, 0};
         for (int i = 0; i < tiles; ++i) {
           f4 c = *reinterpret_cast<const f4*>(cs + 16 * i + 4 * g);
@@ -726,10 +737,11 @@ __global__ __launch_bounds__(kThreads, 2) void attn_weights_kernel(CacheArgs a) 
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) sum[q] = sum_xor32(sum_xor16(sum[q]));
-        const float mine = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
-        if (there && j < sg.len && j < a.span) weights[j] = was + mine;
+        mine = g == 0 ? sum[0] : g == 1 ? sum[1] : g == 2 ? sum[2] : sum[3];
+        at = there && j < sg.len ? j : a.span;
         ks = ks_next;
       }
+      if (at < a.span) weights[at] = was + mine;
       __syncthreads();
     }
   });
